@@ -11,6 +11,8 @@ Public surface (mirrors the reference's Python API):
   quantize_hidden(x_bf16)        FP8 activation quantiser (e4m3 codes + [56, T] block scales)
   pack_gate / gate_quantize      router GEMM fused with the quantiser: logits + codes + scales
   shared_expert_forward(...)     DeepSeek-V3 shared expert (all tokens, weight 1) on the same kernels
+  route_experts / route_experts_backward  expert router of any size and rule, and its gradient (experts.py)
+  linear_w4, experts_w4          products with 4-bit weights and group scales: one matrix, the routed experts
   make_inputs(cfg, device)       seeded synthetic inputs of the benchmark configurations
   ExpertParallel                 expert-parallel layer over the GPUs of one node (ep.py)
   save_packed / load_packed      packed weights on disk (packed_io.py)
@@ -18,6 +20,7 @@ Public surface (mirrors the reference's Python API):
 """
 from .layer import (_cached_pack, _load_custom_ops, gate_quantize, moe_forward, ops, pack_gate, pack_w13,
                     pack_w2, quantize_hidden, route, run, run_custom, shared_expert_forward, workspace_bytes)
+from .experts import (experts_w4, experts_w4_workspace_bytes, linear_w4, route_experts, route_experts_backward)
 from .synth import CONFIGS, MoEConfig, make_inputs, make_weights, quantile_table
 from ._native import MoEError, device_status, set_wait_limit_ns, wait_limit_ns, workspace_layout
 from .ep import ExpertParallel, balanced_placement, expert_range, owner_of, token_range
@@ -30,4 +33,5 @@ __all__ = [
     "make_inputs", "make_weights", "MoEConfig", "CONFIGS", "quantile_table", "MoEError", "device_status", "set_wait_limit_ns", "wait_limit_ns",
     "workspace_layout", "_cached_pack", "_load_custom_ops", "ExpertParallel", "expert_range",
     "owner_of", "token_range", "balanced_placement", "save_packed", "load_packed", "HostPipeline",
+    "route_experts", "route_experts_backward", "linear_w4", "experts_w4", "experts_w4_workspace_bytes",
 ]

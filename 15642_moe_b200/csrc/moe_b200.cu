@@ -22,6 +22,8 @@
 #include "quant.cuh"
 #include "gate.cuh"
 #include "synth.cuh"
+#include "experts_route.cuh"
+#include "w4.cuh"
 #include "moe_b200.h"
 
 #include <cudaTypedefs.h>
@@ -656,6 +658,117 @@ int moe_gate_quantize(const void* hidden_bf16, const void* gate_packed, int T, f
   const dim3 grid(GATE_KS, (T + TILE_M - 1) / TILE_M);
   gate_quantize_kernel<<<grid, GATE_THREADS, GATE_SMEM, static_cast<cudaStream_t>(stream)>>>(map, args);
   return cuda_check(cudaGetLastError(), "gate_quantize launch");
+}
+
+int moe_route_experts(const void* logits, int dtype, long long row_stride, const float* bias, int T, int E, int top_k,
+                      int score, int n_group, int topk_group, int group_score, int renormalize, float scale, int* idx,
+                      float* w, void* stream) {
+  if (dtype < MOE_F32 || dtype > MOE_F16) return fail(MOE_ERR_INVALID, "moe_route_experts: bad dtype");
+  if (T < 0 || E < 1 || E > RX_MAX_E) return fail(MOE_ERR_INVALID, "moe_route_experts: logits must be [T, E] with 1 <= E <= 1024");
+  if (n_group < 1 || n_group > RX_MAX_GROUPS || E % n_group != 0)
+    return fail(MOE_ERR_INVALID, "moe_route_experts: n_group must divide E and be at most 32");
+  if (topk_group < 1 || topk_group > n_group) return fail(MOE_ERR_INVALID, "moe_route_experts: topk_group must be 1 to n_group");
+  if (top_k < 1 || top_k > RX_MAX_K || top_k > E / n_group * topk_group)
+    return fail(MOE_ERR_INVALID, "moe_route_experts: top_k must be 1 to 32 and at most the experts of topk_group groups");
+  if (score < 0 || score > 1 || group_score < 0 || group_score > 1)
+    return fail(MOE_ERR_INVALID, "moe_route_experts: score and group_score must be 0 or 1");
+  if (n_group > 1 && group_score == 1 && E / n_group < 2)
+    return fail(MOE_ERR_INVALID, "moe_route_experts: the sum of the two best needs two experts per group");
+  if (T == 0) return MOE_OK;
+  if (!logits || !idx || !w) return fail(MOE_ERR_INVALID, "moe_route_experts: null pointer argument");
+  const RouteExpertsArgs a{logits, row_stride, bias, T, E, top_k, n_group, topk_group, group_score, score,
+                           renormalize != 0, scale, idx, w};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == MOE_F32) launch_route_experts_t<float>(a, st);
+  else if (dtype == MOE_BF16) launch_route_experts_t<__nv_bfloat16>(a, st);
+  else launch_route_experts_t<__half>(a, st);
+  return cuda_check(cudaGetLastError(), "route_experts launch");
+}
+
+int moe_route_experts_backward(const float* grad_w, const void* logits, int dtype, long long row_stride, const int* idx,
+                               int T, int E, int top_k, int score, int renormalize, float scale, void* grad_logits,
+                               void* stream) {
+  if (dtype < MOE_F32 || dtype > MOE_F16) return fail(MOE_ERR_INVALID, "moe_route_experts_backward: bad dtype");
+  if (T < 0 || E < 1 || E > RX_MAX_E)
+    return fail(MOE_ERR_INVALID, "moe_route_experts_backward: logits must be [T, E] with 1 <= E <= 1024");
+  if (top_k < 1 || top_k > RX_MAX_K) return fail(MOE_ERR_INVALID, "moe_route_experts_backward: top_k must be 1 to 32");
+  if (score < 0 || score > 1) return fail(MOE_ERR_INVALID, "moe_route_experts_backward: score must be 0 or 1");
+  if (T == 0) return MOE_OK;
+  if (!grad_w || !logits || !idx || !grad_logits)
+    return fail(MOE_ERR_INVALID, "moe_route_experts_backward: null pointer argument");
+  const RouteExpertsBwdArgs a{grad_w, logits, row_stride, idx, T, E, top_k, score, renormalize != 0, scale, grad_logits};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == MOE_F32) launch_route_experts_backward_t<float>(a, st);
+  else if (dtype == MOE_BF16) launch_route_experts_backward_t<__nv_bfloat16>(a, st);
+  else launch_route_experts_backward_t<__half>(a, st);
+  return cuda_check(cudaGetLastError(), "route_experts_backward launch");
+}
+
+size_t moe_linear_w4_workspace_bytes(int M, int N, int K) {
+  (void)M; (void)N; (void)K;
+  return 0;
+}
+
+int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* codes, const void* scale, const void* zero,
+                  int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  (void)workspace; (void)workspace_bytes;
+  if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be bf16 or f16");
+  if (M < 0 || N < 1 || K < 1) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be [M, K] and W [N, K]");
+  if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_linear_w4: group must be 32, 64 or 128");
+  if (M == 0) return MOE_OK;
+  if (!x || !codes || !scale || !out) return fail(MOE_ERR_INVALID, "moe_linear_w4: null pointer argument");
+  const W4Matrix w{static_cast<const uint8_t*>(codes), scale, static_cast<const uint8_t*>(zero), group};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long blocks = (static_cast<long long>(M) * N + 7) / 8;
+  if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "moe_linear_w4: M * N is too large");
+  if (dtype == MOE_BF16)
+    linear_w4_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(x), x_stride, w, M, N, K, static_cast<__nv_bfloat16*>(out));
+  else
+    linear_w4_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const __half*>(x), x_stride, w, M, N, K,
+                                                                      static_cast<__half*>(out));
+  return cuda_check(cudaGetLastError(), "linear_w4 launch");
+}
+
+size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I) {
+  if (T < 0 || T > MAX_TOKENS || top_k < 1 || top_k > RX_MAX_K || E < 1 || E > RX_MAX_E || H < 1 || I < 1) return 0;
+  return sizeof(float) * static_cast<size_t>(T) * top_k * I;
+}
+
+int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx, const float* w, const void* w13,
+                   const void* w13_scale, const void* w13_zero, const void* w2, const void* w2_scale,
+                   const void* w2_zero, int group, int T, int top_k, int E, int local_offset, int H, int I, void* out,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_experts_w4: x must be bf16 or f16");
+  if (T < 0 || T > MAX_TOKENS) return fail(MOE_ERR_INVALID, "moe_experts_w4: T must be 0 to 65536");
+  if (top_k < 1 || top_k > RX_MAX_K) return fail(MOE_ERR_INVALID, "moe_experts_w4: top_k must be 1 to 32");
+  if (E < 1 || E > RX_MAX_E) return fail(MOE_ERR_INVALID, "moe_experts_w4: E must be 1 to 1024");
+  if (H < 1 || I < 1) return fail(MOE_ERR_INVALID, "moe_experts_w4: H and I must be at least 1");
+  if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_experts_w4: group must be 32, 64 or 128");
+  if (T == 0) return MOE_OK;
+  if (!x || !idx || !w || !w13 || !w13_scale || !w2 || !w2_scale || !out || !workspace)
+    return fail(MOE_ERR_INVALID, "moe_experts_w4: null pointer argument");
+  const size_t need = moe_experts_w4_workspace_bytes(T, top_k, E, H, I);
+  if (workspace_bytes < need)
+    return fail(MOE_ERR_WORKSPACE, "moe_experts_w4: workspace too small: need " + std::to_string(need) + " bytes");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(MOE_ERR_INVALID, "moe_experts_w4: workspace must be 256-byte aligned");
+  const ExpertsW4Args a{x, x_stride, idx, w,
+                        {static_cast<const uint8_t*>(w13), w13_scale, static_cast<const uint8_t*>(w13_zero), group},
+                        {static_cast<const uint8_t*>(w2), w2_scale, static_cast<const uint8_t*>(w2_zero), group},
+                        T, top_k, E, local_offset, H, I};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* h = static_cast<float*>(workspace);
+  const unsigned up = static_cast<unsigned>((static_cast<long long>(T) * top_k * I + 7) / 8);
+  const unsigned down = static_cast<unsigned>((static_cast<long long>(T) * H + 7) / 8);
+  if (dtype == MOE_BF16) {
+    experts_w4_up_kernel<__nv_bfloat16><<<up, 256, 0, st>>>(a, h);
+    experts_w4_down_kernel<__nv_bfloat16><<<down, 256, 0, st>>>(a, h, static_cast<__nv_bfloat16*>(out));
+  } else {
+    experts_w4_up_kernel<__half><<<up, 256, 0, st>>>(a, h);
+    experts_w4_down_kernel<__half><<<down, 256, 0, st>>>(a, h, static_cast<__half*>(out));
+  }
+  return cuda_check(cudaGetLastError(), "experts_w4 launch");
 }
 
 int moe_synth_logits(const float* table, uint64_t seed, int T, int E, float* out, void* stream) {

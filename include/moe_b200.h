@@ -198,6 +198,52 @@ int moe_pack_gate(const void* w_gate_bf16, void* gate_packed, void* stream);
 int moe_gate_quantize(const void* hidden_bf16, const void* gate_packed, int T, float* logits,
                       void* out_e4m3, float* out_scale, void* stream);
 
+/* ---- Expert router of any size and rule, its gradient, products with 4-bit weights ----
+ * No reference counterparts: the reference has one fixed router and FP8 experts. Element types: */
+#define MOE_F32 0
+#define MOE_BF16 1
+#define MOE_F16 2
+
+/* Router: logits [T, E] of `dtype` (any of the three), rows `row_stride` elements apart -> the top_k experts of each
+ * token in descending order of the choice, ties to the lower expert (idx int32 [T, top_k]) and their
+ * weights (w fp32 [T, top_k]).
+ *   score        0 sigmoid of each logit, 1 softmax of the row
+ *   bias         fp32 [E] added to the scores for the choice only; may be NULL
+ *   n_group      groups of E / n_group neighbouring experts, of which the topk_group best stay;
+ *   group_score  0 a group's best pick, 1 the sum of its two best
+ *   renormalize  != 0: the weights are divided by their sum + 1e-20; then multiplied by `scale`
+ * A logit or bias of -inf excludes an expert; where none is left idx is -1 and the weight 0. NaN logits give NaN
+ * weights. 1 <= E <= 1024, top_k <= 32, n_group <= 32. Any alignment. */
+int moe_route_experts(const void* logits, int dtype, long long row_stride, const float* bias, int T, int E, int top_k,
+                      int score, int n_group, int topk_group, int group_score, int renormalize, float scale, int* idx,
+                      float* w, void* stream);
+
+/* Gradient of moe_route_experts' weights: grad_w fp32 [T, top_k], the forward call's logits and idx (distinct
+ * per row; values outside [0, E) take no part) -> grad_logits [T, E] contiguous, of the logits' type. */
+int moe_route_experts_backward(const float* grad_w, const void* logits, int dtype, long long row_stride, const int* idx,
+                               int T, int E, int top_k, int score, int renormalize, float scale, void* grad_logits,
+                               void* stream);
+
+/* 4-bit weights of a matrix [N, K]: codes [N, ceil(K / 2)] bytes, the even column in the low nibble; scale
+ * [N, ceil(K / group)] of the activations' type (MOE_BF16 or MOE_F16); zero uint8 of the same shape (low four
+ * bits), or NULL for 8; group 32, 64 or 128. Weight = scale * (code - zero). Stacked matrices follow one another.
+ *
+ * moe_linear_w4: out [M, N] = x . W^T, x [M, K] with rows x_stride elements apart, out contiguous; both of type
+ * `dtype`. Sums in fp32, rounded once. */
+size_t moe_linear_w4_workspace_bytes(int M, int N, int K);
+int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* codes, const void* scale, const void* zero,
+                  int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Routed experts with 4-bit weights: for every token t and pick j whose expert e = idx[t, j] - local_offset is in
+ * [0, E): out[t] += w[t, j] * W2[e] (X1 * silu(X2)), [X1 | X2] = W13[e] x[t]. x [T, H] with rows x_stride
+ * elements apart; idx int32 and w fp32 [T, top_k]; w13 stacked [E, 2 I, H], w2 stacked [E, H, I]; out [T, H]
+ * contiguous, of x's type (zeros for a token without a pick here). 0 <= T <= 65536, top_k <= 32, E <= 1024. */
+size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I);
+int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx, const float* w, const void* w13,
+                   const void* w13_scale, const void* w13_zero, const void* w2, const void* w2_scale,
+                   const void* w2_zero, int group, int T, int top_k, int E, int local_offset, int H, int I, void* out,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Seeded synthetic inputs on the GPU (bit-identical to the CPU generator) ----
  * table: device fp32 [65537] inverse-normal-CDF table (see the Python package).
  * No reference counterpart: the reference draws inputs with torch (moe_layer.py:47-74). */
