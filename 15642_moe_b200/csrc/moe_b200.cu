@@ -24,6 +24,7 @@
 #include "synth.cuh"
 #include "experts_route.cuh"
 #include "w4.cuh"
+#include "w4_stream.cuh"
 #include "moe_b200.h"
 
 #include <cudaTypedefs.h>
@@ -704,14 +705,8 @@ int moe_route_experts_backward(const float* grad_w, const void* logits, int dtyp
   return cuda_check(cudaGetLastError(), "route_experts_backward launch");
 }
 
-size_t moe_linear_w4_workspace_bytes(int M, int N, int K) {
-  (void)M; (void)N; (void)K;
-  return 0;
-}
-
 int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* codes, const void* scale, const void* zero,
-                  int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace; (void)workspace_bytes;
+                  int group, int M, int N, int K, void* out, void* stream) {
   if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be bf16 or f16");
   if (M < 0 || N < 1 || K < 1) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be [M, K] and W [N, K]");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_linear_w4: group must be 32, 64 or 128");
@@ -719,6 +714,21 @@ int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* code
   if (!x || !codes || !scale || !out) return fail(MOE_ERR_INVALID, "moe_linear_w4: null pointer argument");
   const W4Matrix w{static_cast<const uint8_t*>(codes), scale, static_cast<const uint8_t*>(zero), group};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M <= WS_TOK) {
+    DeviceInfo* d = nullptr;
+    if (int rc = device_info(&d)) return rc;
+    const int steps = (K + WS_STEP - 1) / WS_STEP, tiles = (N + WS_ROWS - 1) / WS_ROWS;
+    // Split the columns over a cluster until there are two blocks per SM, with two steps each at least.
+    int cluster = 1;
+    while (cluster < 8 && tiles * cluster < 2 * d->num_sms && steps >= 4 * cluster) cluster *= 2;
+    StreamArgs a{x, x_stride, w, M, N, K, 1, 0, 0, nullptr, nullptr, 0, 1, 0, nullptr, out};
+    a.parts = cluster > (steps + WS_CHUNK - 1) / WS_CHUNK ? cluster : (steps + WS_CHUNK - 1) / WS_CHUNK;
+    a.spp = (steps + a.parts - 1) / a.parts;
+    a.parts = (steps + a.spp - 1) / a.spp;
+    return cuda_check(dtype == MOE_BF16 ? launch_w4_stream<__nv_bfloat16, WS_LINEAR>(a, cluster, 1, false, st)
+                                        : launch_w4_stream<__half, WS_LINEAR>(a, cluster, 1, false, st),
+                      "linear_w4 launch");
+  }
   const long long blocks = (static_cast<long long>(M) * N + 7) / 8;
   if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "moe_linear_w4: M * N is too large");
   if (dtype == MOE_BF16)
@@ -732,7 +742,8 @@ int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* code
 
 size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I) {
   if (T < 0 || T > MAX_TOKENS || top_k < 1 || top_k > RX_MAX_K || E < 1 || E > RX_MAX_E || H < 1 || I < 1) return 0;
-  return sizeof(float) * static_cast<size_t>(T) * top_k * I;
+  // Up to 8 tokens: an [T, I] block of intermediate values per pick; else one row per pick.
+  return sizeof(float) * static_cast<size_t>(T) * top_k * I * (T <= WS_TOK ? T : 1);
 }
 
 int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx, const float* w, const void* w13,
@@ -759,6 +770,31 @@ int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx,
                         T, top_k, E, local_offset, H, I};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* h = static_cast<float*>(workspace);
+  if (T <= WS_TOK) {
+    auto split = [&](StreamArgs& b, int at_least) {
+      const int steps = (b.K + WS_STEP - 1) / WS_STEP, need_parts = (steps + WS_CHUNK - 1) / WS_CHUNK;
+      b.parts = at_least > need_parts ? at_least : need_parts;
+      if (b.parts > steps) b.parts = steps;
+      b.spp = (steps + b.parts - 1) / b.parts;
+      b.parts = (steps + b.spp - 1) / b.spp;
+    };
+    // First product: the columns of a pick's expert over a cluster, at most 16 steps per block.
+    StreamArgs up{x, x_stride, a.w13, T, I, H, 1, 0, 0, idx, w, top_k, E, local_offset, h, nullptr};
+    const int steps = (H + WS_STEP - 1) / WS_STEP;
+    int cluster = 1;
+    while (cluster < 8 && steps > WS_CHUNK * cluster) cluster *= 2;
+    split(up, cluster);
+    // Second product: the active experts' columns over a cluster of 8.
+    StreamArgs down{nullptr, 0, a.w2, T, H, I, 1, 0, 0, idx, w, top_k, E, local_offset, h, out};
+    split(down, 1);
+    if (int rc = cuda_check(dtype == MOE_BF16 ? launch_w4_stream<__nv_bfloat16, WS_UP>(up, cluster, T * top_k, false, st)
+                                              : launch_w4_stream<__half, WS_UP>(up, cluster, T * top_k, false, st),
+                            "experts_w4 first product"))
+      return rc;
+    return cuda_check(dtype == MOE_BF16 ? launch_w4_stream<__nv_bfloat16, WS_DOWN>(down, 8, 1, true, st)
+                                        : launch_w4_stream<__half, WS_DOWN>(down, 8, 1, true, st),
+                      "experts_w4 second product");
+  }
   const unsigned up = static_cast<unsigned>((static_cast<long long>(T) * top_k * I + 7) / 8);
   const unsigned down = static_cast<unsigned>((static_cast<long long>(T) * H + 7) / 8);
   if (dtype == MOE_BF16) {

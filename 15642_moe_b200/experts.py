@@ -164,7 +164,7 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: t
                "out must be a contiguous [M, N] tensor of x's type on its device")
     if M:
         _call(_native.cuda_lib().moe_linear_w4, dev, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), codes.data_ptr(),
-              scale.data_ptr(), None if zero is None else zero.data_ptr(), group, M, N, K, out.data_ptr(), None, 0)
+              scale.data_ptr(), None if zero is None else zero.data_ptr(), group, M, N, K, out.data_ptr())
     return out
 
 

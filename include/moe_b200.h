@@ -230,9 +230,8 @@ int moe_route_experts_backward(const float* grad_w, const void* logits, int dtyp
  *
  * moe_linear_w4: out [M, N] = x . W^T, x [M, K] with rows x_stride elements apart, out contiguous; both of type
  * `dtype`. Sums in fp32, rounded once. */
-size_t moe_linear_w4_workspace_bytes(int M, int N, int K);
 int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* codes, const void* scale, const void* zero,
-                  int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream);
+                  int group, int M, int N, int K, void* out, void* stream);
 
 /* Routed experts with 4-bit weights: for every token t and pick j whose expert e = idx[t, j] - local_offset is in
  * [0, E): out[t] += w[t, j] * W2[e] (X1 * silu(X2)), [X1 | X2] = W13[e] x[t]. x [T, H] with rows x_stride

@@ -41,7 +41,7 @@ def test_router_refuses(lib, ptr):
 def test_products_refuse(lib, ptr):
     p = ptr[0]
     call = lambda dtype=1, group=128, M=2, N=8, K=64, x=p: lib.moe_linear_w4(  # noqa: E731
-        x, dtype, 64, p, p, None, group, M, N, K, p, None, 0, None)
+        x, dtype, 64, p, p, None, group, M, N, K, p, None)
     for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=16), b"group"), (dict(M=-1), b"[M, K]"), (dict(N=0), b"[M, K]"),
                      (dict(K=0), b"[M, K]"), (dict(x=None), b"null")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
