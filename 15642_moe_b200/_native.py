@@ -70,8 +70,9 @@ CUDA_SIGNATURES = {
                                   c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),
     "moe_route_experts_backward": (c_int, [c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int, c_int, c_int,
                                            c_int, c_int, c_float, c_void_p, c_void_p]),
+    "moe_linear_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "moe_linear_w4": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                              c_void_p, c_void_p]),
+                              c_void_p, c_void_p, c_size_t, c_void_p]),
     "moe_experts_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "moe_experts_w4": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,

@@ -26,7 +26,7 @@ SYNTH_CPU_LIB = os.path.join(PKG_DIR, "libmoe_synth_cpu.so")
 
 CUDA_SOURCES = ["moe_b200.cu"]
 CUDA_HEADERS = ["moe_common.cuh", "route.cuh", "ep.cuh", "gemm1.cuh", "gemm2.cuh", "pack.cuh", "quant.cuh", "gate.cuh", "synth.cuh",
-                "experts_route.cuh", "w4.cuh", "w4_stream.cuh",
+                "experts_route.cuh", "w4.cuh", "w4_stream.cuh", "w4_mma.cuh",
                 "synth_core.h"]
 
 NVCC_FLAGS = [

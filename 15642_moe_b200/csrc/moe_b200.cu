@@ -25,10 +25,12 @@
 #include "experts_route.cuh"
 #include "w4.cuh"
 #include "w4_stream.cuh"
+#include "w4_mma.cuh"
 #include "moe_b200.h"
 
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cstring>
 #include <mutex>
 #include <utility>
@@ -661,6 +663,261 @@ int moe_gate_quantize(const void* hidden_bf16, const void* gate_packed, int T, f
   return cuda_check(cudaGetLastError(), "gate_quantize launch");
 }
 
+}  // extern "C"
+
+namespace {
+
+// ---- 4-bit products ------------------------------------------------------------------------
+
+int round_up(long long v, int to) { return static_cast<int>((v + to - 1) / to * to); }
+int w4_bytes(int K) { return static_cast<int>((static_cast<long long>(K) + 1) / 2); }
+// TMA wants rows that start on 16-byte boundaries.
+bool w4_rows_aligned(const void* codes, int K) { return w4_bytes(K) % 16 == 0 && aligned16(codes); }
+
+// Tokens per tile: the accumulators are as small as the largest expected tile allows, so that more of them fit.
+int wm_tile(long long rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+constexpr int WM_SMS = 148;   // the split rule's SM count: results and workspace sizes do not depend on the device
+
+// linear_w4: parts of the columns, so that few row tiles still fill the SMs; four steps of 128 each at least.
+int wm_splits(int M, int N, int K) {
+  const long long nt = wm_tile(M), units = (M + nt - 1) / nt * ((N + 127ll) / 128);
+  const int steps = (K + 127) / 128;
+  long long s = WM_SMS / units;
+  if (s > steps / 4) s = steps / 4;
+  if (s > 16) s = 16;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+struct LinearW4Ws {
+  size_t x, parts, codes, total;
+};
+LinearW4Ws make_linear_w4_ws(int M, int N, int K) {
+  LinearW4Ws w{};
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t o = off;
+    off = ws_align(off + n);
+    return o;
+  };
+  w.x = take(static_cast<size_t>(M) * round_up(K, 8) * 2);
+  const int splits = wm_splits(M, N, K);
+  w.parts = take(splits > 1 ? sizeof(float) * splits * static_cast<size_t>(M) * N : 0);
+  // The copy of the codes is only used where their own rows do not allow TMA; a base that is not 16-byte aligned
+  // can make any shape need it.
+  w.codes = take(static_cast<size_t>(N) * round_up(w4_bytes(K), 16));
+  w.total = off;
+  return w;
+}
+
+struct ExpertsW4Ws {
+  size_t h8;                                     // up to 8 tokens: fp32 [T k][T][I]
+  size_t counts, slot, x, h, y, c13, c2, total;  // more
+};
+ExpertsW4Ws make_experts_w4_ws(int T, int k, int E, int H, int I) {
+  ExpertsW4Ws w{};
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t o = off;
+    off = ws_align(off + n);
+    return o;
+  };
+  const size_t routes = static_cast<size_t>(T) * k;
+  if (T <= WS_TOK) {
+    w.h8 = take(sizeof(float) * routes * T * I);
+  } else {
+    w.counts = take(sizeof(int) * E);
+    w.slot = take(sizeof(int) * routes);
+    w.x = take(routes * round_up(H, 8) * 2);
+    w.h = take(routes * round_up(I, 8) * 4);
+    w.y = take(routes * H * 4);
+    // Copies of codes whose rows do not allow TMA (odd widths).
+    w.c13 = take(w4_bytes(H) % 16 ? static_cast<size_t>(E) * 2 * I * round_up(w4_bytes(H), 16) : 0);
+    w.c2 = take(w4_bytes(I) % 16 ? static_cast<size_t>(E) * H * round_up(w4_bytes(I), 16) : 0);
+  }
+  w.total = off;
+  return w;
+}
+
+// Tensor map of a 2-D array of rows `pitch` bytes apart, 128-byte swizzle, boxes of 128 bytes x `box_rows`.
+int w4_map(CUtensorMapDataType type, const void* base, long long width, long long rows, long long pitch, int box_width, int box_rows,
+           CUtensorMap* map) {
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  if (encode == nullptr) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_width), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(r));
+  return MOE_OK;
+}
+
+// Shared-memory opt-in and the register check of one kernel, once per device.
+template <auto kernel>
+int wm_prepare(int smem, bool split_regs) {
+  static std::atomic<unsigned char> done[64];
+  int dev = 0;
+  if (int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  if (dev < 0 || dev >= 64) return fail(MOE_ERR_CUDA, "device ordinal out of range");
+  if (done[dev].load(std::memory_order_acquire)) return MOE_OK;
+  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(w4)")) return rc;
+  if (split_regs) {
+    cudaFuncAttributes fa{};
+    if (int rc = cuda_check(cudaFuncGetAttributes(&fa, kernel), "cudaFuncGetAttributes(w4)")) return rc;
+    if (fa.numRegs < WM_LAUNCH_REGS_MIN)
+      return fail(MOE_ERR_CUDA, "w4_mma_kernel built with " + std::to_string(fa.numRegs) + " registers per thread; the split needs " +
+                                    std::to_string(WM_LAUNCH_REGS_MIN));
+  }
+  done[dev].store(1, std::memory_order_release);
+  return MOE_OK;
+}
+
+template <typename T, int MODE, int NT>
+int launch_w4_mma_nt(DeviceInfo* d, const CUtensorMap& cm, const CUtensorMap& xm, const WmArgs& a, long long units, cudaStream_t st) {
+  if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT>>(WM_SMEM<NT>, NT == 128)) return rc;
+  const int grid = units < d->num_sms ? static_cast<int>(units) : d->num_sms;
+  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT>, grid < 1 ? 1 : grid, WM_THREADS, WM_SMEM<NT>, st, cm, xm, a),
+                    "w4_mma launch");
+}
+
+// `rows`: tokens (routes) in the x buffer, each `width` columns; tile: expected tokens of one expert.
+template <typename T, int MODE>
+int launch_w4_mma(DeviceInfo* d, const WmArgs& a, const void* x, long long x_rows, int tile, cudaStream_t st) {
+  const int pitch = round_up(w4_bytes(a.K), 16), width = round_up(a.K, 8);
+  const long long rows = static_cast<long long>(a.E) * (MODE == WS_UP ? 2 : 1) * a.N;
+  CUtensorMap cm, xm;
+  if (int rc = w4_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w.codes, pitch, rows, pitch, 128, 64, &cm)) return rc;
+  const CUtensorMapDataType t = MODE != WS_DOWN && std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, WM_BOX_TOK, &xm)) return rc;
+  const int per = MODE == WS_UP ? 64 : 128;
+  // Most units that there can be: every expert's tokens in tiles, or one token in each.
+  const long long row_tiles = (static_cast<long long>(a.N) + per - 1) / per;
+  const long long tokens = MODE == WS_LINEAR ? a.M : a.row_cap;
+  const long long tiles = MODE == WS_LINEAR ? (tokens + tile - 1) / tile : (tokens < a.E ? tokens : a.E) + tokens / tile;
+  const long long units = tiles * row_tiles * a.splits;
+  switch (tile) {
+    case 32: return launch_w4_mma_nt<T, MODE, 32>(d, cm, xm, a, units, st);
+    case 64: return launch_w4_mma_nt<T, MODE, 64>(d, cm, xm, a, units, st);
+    default: return launch_w4_mma_nt<T, MODE, 128>(d, cm, xm, a, units, st);
+  }
+}
+
+// Codes as TMA can read them: the caller's, or a copy with padded rows.
+int w4_tma_codes(DeviceInfo* d, const uint8_t* codes, long long rows, int K, uint8_t* copy, const uint8_t** out, cudaStream_t st) {
+  *out = codes;
+  if (w4_rows_aligned(codes, K)) return MOE_OK;
+  const int bytes = w4_bytes(K), pitch = round_up(bytes, 16);
+  pad_codes_kernel<<<grid_for(static_cast<size_t>(rows) * (pitch / 4), 256, d->num_sms * 16), 256, 0, st>>>(codes, rows, bytes, pitch, copy);
+  *out = copy;
+  return cuda_check(cudaGetLastError(), "pad_codes launch");
+}
+
+template <typename T>
+int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Matrix& w, int M, int N, int K, void* out, void* workspace,
+                   cudaStream_t st) {
+  if (M <= WS_TOK) {
+    const int steps = (K + WS_STEP - 1) / WS_STEP, tiles = (N + WS_ROWS - 1) / WS_ROWS;
+    // Split the columns over a cluster until there are two blocks per SM, with two steps each at least.
+    int cluster = 1;
+    while (cluster < 8 && tiles * cluster < 2 * d->num_sms && steps >= 4 * cluster) cluster *= 2;
+    StreamArgs a{x, x_stride, w, M, N, K, 1, 0, 0, nullptr, nullptr, 0, 1, 0, nullptr, out};
+    a.parts = cluster > (steps + WS_CHUNK - 1) / WS_CHUNK ? cluster : (steps + WS_CHUNK - 1) / WS_CHUNK;
+    a.spp = (steps + a.parts - 1) / a.parts;
+    a.parts = (steps + a.spp - 1) / a.spp;
+    return cuda_check(launch_w4_stream<T, WS_LINEAR>(a, cluster, 1, false, st), "linear_w4 launch");
+  }
+  const LinearW4Ws ws = make_linear_w4_ws(M, N, K);
+  uint8_t* W = static_cast<uint8_t*>(workspace);
+  WmArgs a{};
+  a.w = w;
+  if (int rc = w4_tma_codes(d, w.codes, N, K, W + ws.codes, &a.w.codes, st)) return rc;
+  pair_rows_kernel<T><<<grid_for(static_cast<size_t>(M) * (round_up(K, 8) / 8), 256, d->num_sms * 8), 256, 0, st>>>(
+      static_cast<const T*>(x), x_stride, M, K, reinterpret_cast<T*>(W + ws.x));
+  a.E = 1;
+  a.N = N;
+  a.K = K;
+  a.M = M;
+  a.row_cap = M;
+  a.splits = wm_splits(M, N, K);
+  a.sps = round_up((static_cast<long long>((K + 127) / 128) + a.splits - 1) / a.splits, 2);
+  a.splits = ((K + 127) / 128 + a.sps - 1) / a.sps;
+  a.y = reinterpret_cast<float*>(W + ws.parts);
+  a.out = out;
+  if (int rc = launch_w4_mma<T, WS_LINEAR>(d, a, W + ws.x, M, wm_tile(M), st)) return rc;
+  if (a.splits > 1) {
+    const long long n = static_cast<long long>(M) * N;
+    return cuda_check(launch_programmatic(sum_parts_kernel<T>, grid_for(static_cast<size_t>(n), 256, d->num_sms * 8), 256, 0, st,
+                                          static_cast<const float*>(a.y), a.splits, n, static_cast<T*>(out)),
+                      "sum_parts launch");
+  }
+  return MOE_OK;
+}
+
+template <typename T>
+int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W, cudaStream_t st) {
+  const ExpertsW4Ws ws = make_experts_w4_ws(p.T, p.k, p.E, p.H, p.I);
+  if (p.T <= WS_TOK) {
+    float* h = reinterpret_cast<float*>(W + ws.h8);
+    auto split = [&](StreamArgs& b, int at_least) {
+      const int steps = (b.K + WS_STEP - 1) / WS_STEP, need_parts = (steps + WS_CHUNK - 1) / WS_CHUNK;
+      b.parts = at_least > need_parts ? at_least : need_parts;
+      if (b.parts > steps) b.parts = steps;
+      b.spp = (steps + b.parts - 1) / b.parts;
+      b.parts = (steps + b.spp - 1) / b.spp;
+    };
+    // First product: the columns of a pick's expert over a cluster, at most 16 steps per block.
+    StreamArgs up{p.x, p.x_stride, p.w13, p.T, p.I, p.H, 1, 0, 0, p.idx, p.wt, p.k, p.E, p.offset, h, nullptr};
+    const int steps = (p.H + WS_STEP - 1) / WS_STEP;
+    int cluster = 1;
+    while (cluster < 8 && steps > WS_CHUNK * cluster) cluster *= 2;
+    split(up, cluster);
+    // Second product: the active experts' columns over a cluster of 8.
+    StreamArgs down{nullptr, 0, p.w2, p.T, p.H, p.I, 1, 0, 0, p.idx, p.wt, p.k, p.E, p.offset, h, out};
+    split(down, 1);
+    if (int rc = cuda_check(launch_w4_stream<T, WS_UP>(up, cluster, p.T * p.k, false, st), "experts_w4 first product")) return rc;
+    return cuda_check(launch_w4_stream<T, WS_DOWN>(down, 8, 1, true, st), "experts_w4 second product");
+  }
+  const int routes = p.T * p.k;
+  int* counts = reinterpret_cast<int*>(W + ws.counts);
+  int* slot = reinterpret_cast<int*>(W + ws.slot);
+  T* xg = reinterpret_cast<T*>(W + ws.x);
+  __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(W + ws.h);
+  float* y = reinterpret_cast<float*>(W + ws.y);
+  WmArgs up{}, down{};
+  up.w = p.w13;
+  down.w = p.w2;
+  if (int rc = w4_tma_codes(d, p.w13.codes, 2ll * p.E * p.I, p.H, W + ws.c13, &up.w.codes, st)) return rc;
+  if (int rc = w4_tma_codes(d, p.w2.codes, static_cast<long long>(p.E) * p.H, p.I, W + ws.c2, &down.w.codes, st)) return rc;
+  if (int rc = cuda_check(cudaMemsetAsync(counts, 0, sizeof(int) * p.E, st), "memset counts")) return rc;
+  experts_slot_kernel<<<grid_for(static_cast<size_t>(routes), 256, d->num_sms * 4), 256, 0, st>>>(p.idx, routes, p.offset, p.E, counts, slot);
+  experts_gather_kernel<T><<<grid_for(static_cast<size_t>(routes), 8, d->num_sms * 8), 256, 0, st>>>(
+      static_cast<const T*>(p.x), p.x_stride, p.idx, routes, p.k, p.offset, p.E, counts, p.H, slot, xg);
+  up.E = down.E = p.E;
+  up.counts = down.counts = counts;
+  up.row_cap = down.row_cap = routes;
+  up.splits = down.splits = 1;
+  up.N = down.K = p.I;
+  up.K = down.N = p.H;
+  up.sps = round_up((up.K + 127) / 128, 2);
+  down.sps = round_up((down.K + 127) / 128, 2);
+  up.h = h;
+  up.h_pitch = round_up(p.I, 8);
+  down.y = y;
+  const int tile = wm_tile((routes + p.E - 1) / p.E);
+  if (int rc = launch_w4_mma<T, WS_UP>(d, up, xg, routes, tile, st)) return rc;
+  if (int rc = launch_w4_mma<T, WS_DOWN>(d, down, h, 2ll * routes, tile, st)) return rc;
+  return cuda_check(launch_programmatic(experts_combine_kernel<T>, grid_for(static_cast<size_t>(p.T) * p.H, 256, d->num_sms * 16), 256, 0, st,
+                                        static_cast<const float*>(y), static_cast<const int*>(slot), p.wt, p.T, p.k, p.H,
+                                        static_cast<T*>(out)),
+                    "experts_combine launch");
+}
+
+}  // namespace
+
+extern "C" {
+
 int moe_route_experts(const void* logits, int dtype, long long row_stride, const float* bias, int T, int E, int top_k,
                       int score, int n_group, int topk_group, int group_score, int renormalize, float scale, int* idx,
                       float* w, void* stream) {
@@ -705,8 +962,13 @@ int moe_route_experts_backward(const float* grad_w, const void* logits, int dtyp
   return cuda_check(cudaGetLastError(), "route_experts_backward launch");
 }
 
+size_t moe_linear_w4_workspace_bytes(int M, int N, int K) {
+  if (M <= WS_TOK || N < 1 || K < 1) return 0;
+  return make_linear_w4_ws(M, N, K).total;
+}
+
 int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* codes, const void* scale, const void* zero,
-                  int group, int M, int N, int K, void* out, void* stream) {
+                  int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be bf16 or f16");
   if (M < 0 || N < 1 || K < 1) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be [M, K] and W [N, K]");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_linear_w4: group must be 32, 64 or 128");
@@ -714,36 +976,22 @@ int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* code
   if (!x || !codes || !scale || !out) return fail(MOE_ERR_INVALID, "moe_linear_w4: null pointer argument");
   const W4Matrix w{static_cast<const uint8_t*>(codes), scale, static_cast<const uint8_t*>(zero), group};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M <= WS_TOK) {
-    DeviceInfo* d = nullptr;
-    if (int rc = device_info(&d)) return rc;
-    const int steps = (K + WS_STEP - 1) / WS_STEP, tiles = (N + WS_ROWS - 1) / WS_ROWS;
-    // Split the columns over a cluster until there are two blocks per SM, with two steps each at least.
-    int cluster = 1;
-    while (cluster < 8 && tiles * cluster < 2 * d->num_sms && steps >= 4 * cluster) cluster *= 2;
-    StreamArgs a{x, x_stride, w, M, N, K, 1, 0, 0, nullptr, nullptr, 0, 1, 0, nullptr, out};
-    a.parts = cluster > (steps + WS_CHUNK - 1) / WS_CHUNK ? cluster : (steps + WS_CHUNK - 1) / WS_CHUNK;
-    a.spp = (steps + a.parts - 1) / a.parts;
-    a.parts = (steps + a.spp - 1) / a.spp;
-    return cuda_check(dtype == MOE_BF16 ? launch_w4_stream<__nv_bfloat16, WS_LINEAR>(a, cluster, 1, false, st)
-                                        : launch_w4_stream<__half, WS_LINEAR>(a, cluster, 1, false, st),
-                      "linear_w4 launch");
+  if (M > WS_TOK) {
+    const size_t need = moe_linear_w4_workspace_bytes(M, N, K);
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(MOE_ERR_WORKSPACE, "moe_linear_w4: workspace too small: need " + std::to_string(need) + " bytes");
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+      return fail(MOE_ERR_INVALID, "moe_linear_w4: workspace must be 256-byte aligned");
   }
-  const long long blocks = (static_cast<long long>(M) * N + 7) / 8;
-  if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "moe_linear_w4: M * N is too large");
-  if (dtype == MOE_BF16)
-    linear_w4_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(x), x_stride, w, M, N, K, static_cast<__nv_bfloat16*>(out));
-  else
-    linear_w4_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const __half*>(x), x_stride, w, M, N, K,
-                                                                      static_cast<__half*>(out));
-  return cuda_check(cudaGetLastError(), "linear_w4 launch");
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  return dtype == MOE_BF16 ? linear_w4_impl<__nv_bfloat16>(d, x, x_stride, w, M, N, K, out, workspace, st)
+                           : linear_w4_impl<__half>(d, x, x_stride, w, M, N, K, out, workspace, st);
 }
 
 size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I) {
   if (T < 0 || T > MAX_TOKENS || top_k < 1 || top_k > RX_MAX_K || E < 1 || E > RX_MAX_E || H < 1 || I < 1) return 0;
-  // Up to 8 tokens: an [T, I] block of intermediate values per pick; else one row per pick.
-  return sizeof(float) * static_cast<size_t>(T) * top_k * I * (T <= WS_TOK ? T : 1);
+  return make_experts_w4_ws(T, top_k, E, H, I).total;
 }
 
 int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx, const float* w, const void* w13,
@@ -755,10 +1003,13 @@ int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx,
   if (top_k < 1 || top_k > RX_MAX_K) return fail(MOE_ERR_INVALID, "moe_experts_w4: top_k must be 1 to 32");
   if (E < 1 || E > RX_MAX_E) return fail(MOE_ERR_INVALID, "moe_experts_w4: E must be 1 to 1024");
   if (H < 1 || I < 1) return fail(MOE_ERR_INVALID, "moe_experts_w4: H and I must be at least 1");
+  if (static_cast<long long>(E) * (2ll * I > H ? 2ll * I : H) > 0x7FFFFFFFll)
+    return fail(MOE_ERR_INVALID, "moe_experts_w4: the experts' matrices have more than 2^31 rows");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_experts_w4: group must be 32, 64 or 128");
   if (T == 0) return MOE_OK;
   if (!x || !idx || !w || !w13 || !w13_scale || !w2 || !w2_scale || !out || !workspace)
     return fail(MOE_ERR_INVALID, "moe_experts_w4: null pointer argument");
+  if (!aligned16(w13) || !aligned16(w2)) return fail(MOE_ERR_INVALID, "moe_experts_w4: w13 and w2 must be 16-byte aligned");
   const size_t need = moe_experts_w4_workspace_bytes(T, top_k, E, H, I);
   if (workspace_bytes < need)
     return fail(MOE_ERR_WORKSPACE, "moe_experts_w4: workspace too small: need " + std::to_string(need) + " bytes");
@@ -768,43 +1019,11 @@ int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx,
                         {static_cast<const uint8_t*>(w13), w13_scale, static_cast<const uint8_t*>(w13_zero), group},
                         {static_cast<const uint8_t*>(w2), w2_scale, static_cast<const uint8_t*>(w2_zero), group},
                         T, top_k, E, local_offset, H, I};
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* h = static_cast<float*>(workspace);
-  if (T <= WS_TOK) {
-    auto split = [&](StreamArgs& b, int at_least) {
-      const int steps = (b.K + WS_STEP - 1) / WS_STEP, need_parts = (steps + WS_CHUNK - 1) / WS_CHUNK;
-      b.parts = at_least > need_parts ? at_least : need_parts;
-      if (b.parts > steps) b.parts = steps;
-      b.spp = (steps + b.parts - 1) / b.parts;
-      b.parts = (steps + b.spp - 1) / b.spp;
-    };
-    // First product: the columns of a pick's expert over a cluster, at most 16 steps per block.
-    StreamArgs up{x, x_stride, a.w13, T, I, H, 1, 0, 0, idx, w, top_k, E, local_offset, h, nullptr};
-    const int steps = (H + WS_STEP - 1) / WS_STEP;
-    int cluster = 1;
-    while (cluster < 8 && steps > WS_CHUNK * cluster) cluster *= 2;
-    split(up, cluster);
-    // Second product: the active experts' columns over a cluster of 8.
-    StreamArgs down{nullptr, 0, a.w2, T, H, I, 1, 0, 0, idx, w, top_k, E, local_offset, h, out};
-    split(down, 1);
-    if (int rc = cuda_check(dtype == MOE_BF16 ? launch_w4_stream<__nv_bfloat16, WS_UP>(up, cluster, T * top_k, false, st)
-                                              : launch_w4_stream<__half, WS_UP>(up, cluster, T * top_k, false, st),
-                            "experts_w4 first product"))
-      return rc;
-    return cuda_check(dtype == MOE_BF16 ? launch_w4_stream<__nv_bfloat16, WS_DOWN>(down, 8, 1, true, st)
-                                        : launch_w4_stream<__half, WS_DOWN>(down, 8, 1, true, st),
-                      "experts_w4 second product");
-  }
-  const unsigned up = static_cast<unsigned>((static_cast<long long>(T) * top_k * I + 7) / 8);
-  const unsigned down = static_cast<unsigned>((static_cast<long long>(T) * H + 7) / 8);
-  if (dtype == MOE_BF16) {
-    experts_w4_up_kernel<__nv_bfloat16><<<up, 256, 0, st>>>(a, h);
-    experts_w4_down_kernel<__nv_bfloat16><<<down, 256, 0, st>>>(a, h, static_cast<__nv_bfloat16*>(out));
-  } else {
-    experts_w4_up_kernel<__half><<<up, 256, 0, st>>>(a, h);
-    experts_w4_down_kernel<__half><<<down, 256, 0, st>>>(a, h, static_cast<__half*>(out));
-  }
-  return cuda_check(cudaGetLastError(), "experts_w4 launch");
+  return dtype == MOE_BF16 ? experts_w4_impl<__nv_bfloat16>(d, a, out, static_cast<uint8_t*>(workspace), st)
+                           : experts_w4_impl<__half>(d, a, out, static_cast<uint8_t*>(workspace), st);
 }
 
 int moe_synth_logits(const float* table, uint64_t seed, int T, int E, float* out, void* stream) {

@@ -1,0 +1,604 @@
+/*
+ * Products with 4-bit weights for more than a few tokens, on tcgen05.mma (kind::f16): the weights are the
+ * M = 128 operand in tensor memory, the tokens (16 to NT columns) the N operand in shared memory.
+ *
+ *   codes -> TMA, 128 rows x 256 columns a stage -> 8 warps turn a row's codes into numbers code - zero, exact in
+ *   bf16 and f16 (a nibble in the mantissa of 128 or 1024, minus 128 + zero or 1024 + zero) -> tensor memory ->
+ *   one accumulator per group of columns -> 4 warps add scale * accumulator to the row's sums in fp32.
+ *
+ * No weight is rounded, and the scale of a group multiplies a finished sum. A thread owns a weight row all the way:
+ * it reads the row's codes, writes the row's lane of tensor memory, and (in the last warps) scales its sums.
+ *
+ * A word's codes come out as the pairs (0,4), (1,5), (2,6), (3,7) with two instructions each; the tokens' rows are
+ * kept in that order of columns (within each 8), which costs their copy nothing.
+ *
+ * Roles (16 warps): warp 0 loads codes, warp 1 issues the mma, warp 2 loads token rows, warps 4-11 convert (two
+ * warpgroups take turns with steps of 128 columns), warps 12-15 scale and store. Persistent: one block per SM walks
+ * the units (token tile, 128 weight rows[, part of the columns]).
+ */
+#pragma once
+#include "gate.cuh"
+#include "w4_stream.cuh"
+
+namespace moe {
+
+constexpr int WM_THREADS = 512;
+constexpr int WM_CODE_BYTES = 128 * 128;        // 128 rows x 256 columns
+constexpr int WM_B_STAGES = 8;                  // 64 columns of the tile's tokens each
+constexpr int WM_A_SLOTS = 4;                   // steps of 128 columns in tensor memory (64 of its columns each)
+constexpr int WM_A_COL = 256;                   // accumulators in [0, 256), weights in [256, 512)
+constexpr int WM_MAX_BUFS = 4;
+constexpr int WM_BOX_TOK = 16;                  // token rows per TMA box
+constexpr int WM_REGS_CTRL = 48, WM_REGS_CONV = 104, WM_REGS_EPI = 232;   // register split for NT = 128
+constexpr int WM_LAUNCH_REGS_MIN = (WM_REGS_CTRL + 2 * WM_REGS_CONV + WM_REGS_EPI + 3) / 4;
+
+template <int NT>
+struct WmShape {
+  static constexpr int CODE_STAGES = NT == 128 ? 5 : 8;
+  static constexpr int B_BYTES = NT * 128;
+  static constexpr int BUFS = 256 / NT < WM_MAX_BUFS ? 256 / NT : WM_MAX_BUFS;   // accumulators
+  static constexpr int RING = CODE_STAGES * WM_CODE_BYTES + WM_B_STAGES * B_BYTES;
+};
+
+struct WmCtrl {
+  uint64_t c_full[8], c_empty[8];
+  uint64_t b_full[WM_B_STAGES], b_empty[WM_B_STAGES];
+  uint64_t a_full[WM_A_SLOTS], a_empty[WM_A_SLOTS];
+  uint64_t d_full[WM_MAX_BUFS], d_empty[WM_MAX_BUFS];
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort_flag;
+  int tiles, rows;                              // token tiles of all experts; routes
+  int tile_off[RX_MAX_E + 1];                   // first token tile of each expert
+  int row_off[RX_MAX_E + 1];                    // first row of each expert in the route-ordered buffers
+};
+
+template <int NT>
+constexpr int WM_SMEM = WmShape<NT>::RING + static_cast<int>(sizeof(WmCtrl)) + 1024;
+
+struct WmArgs {
+  W4Matrix w;
+  int E, N, K;              // experts; output columns (up: I) and reduction length of one
+  int M;                    // linear: tokens
+  const int* counts;        // [E] routes per expert (up, down)
+  int row_cap;              // rows of the route-ordered buffers
+  int splits, sps;          // linear: parts of the columns, each of `sps` (even) steps of 128
+  __nv_bfloat16* h;         // up: [2][row_cap][Ip] hi and lo of the intermediate, columns in pair order
+  int h_pitch;              // Ip
+  float* y;                 // down: [row_cap][N]; linear with splits: [splits][M][N]
+  void* out;                // linear: [M][N]
+};
+
+// Position of column c inside the pair order (0,4,1,5,2,6,3,7) of its 8, and back.
+__host__ __device__ __forceinline__ int pair_pos(int c) { return (c & ~7) | ((c & 3) << 1) | ((c >> 2) & 1); }
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D(tmem) (+)= A(tmem, 128 x 16) x B(smem desc)^T, bf16 or f16 operands (idesc), fp32 accumulate.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Tiles of up to NT tokens: an expert's rows in equal parts.
+__host__ __device__ __forceinline__ int wm_tiles(int rows, int nt) { return (rows + nt - 1) / nt; }
+
+// Prefix sums of the experts' tiles and rows; one full warp. Counts outside [0, cap], or adding up to more than cap,
+// are reported and taken as none.
+__device__ __forceinline__ void wm_build_map(int* tile_off, int* row_off, const int* counts, int E, int cap, int nt) {
+  const int lane = threadIdx.x & 31, per = (E + 31) / 32;
+  long long rows = 0;
+  int tiles = 0;
+  bool bad = false;
+  for (int i = 0; i < per; ++i) {
+    const int e = lane * per + i;
+    const int c = e < E ? counts[e] : 0;
+    bad |= c < 0 || c > cap;
+    rows += c;
+    tiles += wm_tiles(c, nt);
+  }
+  long long r_incl = rows;
+  int t_incl = tiles;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long rn = __shfl_up_sync(0xffffffffu, r_incl, o);
+    const int tn = __shfl_up_sync(0xffffffffu, t_incl, o);
+    if (lane >= o) {
+      r_incl += rn;
+      t_incl += tn;
+    }
+  }
+  bad = __any_sync(0xffffffffu, bad || r_incl > cap);
+  if (bad && lane == 0) report_status(ST_BAD_INDEX);
+  int t = bad ? 0 : t_incl - tiles, r = bad ? 0 : static_cast<int>(r_incl - rows);
+  for (int i = 0; i < per; ++i) {
+    const int e = lane * per + i;
+    if (e <= E) {
+      tile_off[e] = t;
+      row_off[e] = r;
+    }
+    const int c = e < E && !bad ? counts[e] : 0;
+    t += wm_tiles(c, nt);
+    r += c;
+  }
+  if (lane == 31 && 32 * per == E) {
+    tile_off[E] = t;
+    row_off[E] = r;
+  }
+}
+
+struct WmUnit {
+  int expert, row0, tokens;    // first row and count of the tile's tokens
+  int rt, split;               // 128-row tile of the weights; part of the columns
+};
+
+template <int NT>
+__device__ __forceinline__ WmUnit wm_unit(const WmCtrl* ctl, const WmArgs& p, int u, int row_tiles) {
+  WmUnit w;
+  w.rt = u % row_tiles;
+  int tile = u / row_tiles;
+  w.split = tile % p.splits;
+  tile /= p.splits;
+  int lo = 0, hi = p.E;        // tile_off[lo] <= tile < tile_off[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (ctl->tile_off[mid] <= tile) lo = mid; else hi = mid;
+  }
+  w.expert = lo;
+  const int rows = ctl->row_off[lo + 1] - ctl->row_off[lo], tiles = ctl->tile_off[lo + 1] - ctl->tile_off[lo];
+  const int i = tile - ctl->tile_off[lo];
+  const int a = static_cast<int>(static_cast<long long>(rows) * i / tiles), b = static_cast<int>(static_cast<long long>(rows) * (i + 1) / tiles);
+  w.row0 = ctl->row_off[lo] + a;
+  w.tokens = b - a;
+  return w;
+}
+
+template <typename T, int MODE, int NT>
+__global__ void __launch_bounds__(WM_THREADS, 1)
+    w4_mma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map,
+                  const __grid_constant__ WmArgs p) {
+  using W = typename std::conditional<MODE == WS_DOWN, __nv_bfloat16, T>::type;   // the operands' type
+  using S = WmShape<NT>;
+  constexpr int TERMS = MODE == WS_DOWN ? 2 : 1;
+  extern __shared__ uint8_t wm_raw[];
+  uint8_t* smem = align_1024(wm_raw);
+  uint8_t* ring_c = smem;
+  uint8_t* ring_b = smem + S::CODE_STAGES * WM_CODE_BYTES;
+  WmCtrl* ctl = reinterpret_cast<WmCtrl*>(smem + S::RING);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::CODE_STAGES; ++i) {
+      mbar_init(&ctl->c_full[i], 1);
+      mbar_init(&ctl->c_empty[i], 8);
+    }
+    for (int i = 0; i < WM_B_STAGES; ++i) {
+      mbar_init(&ctl->b_full[i], 1);
+      mbar_init(&ctl->b_empty[i], 1);
+    }
+    for (int i = 0; i < WM_A_SLOTS; ++i) {
+      mbar_init(&ctl->a_full[i], 4);
+      mbar_init(&ctl->a_empty[i], 1);
+    }
+    for (int i = 0; i < S::BUFS; ++i) {
+      mbar_init(&ctl->d_full[i], 1);
+      mbar_init(&ctl->d_empty[i], 4);
+    }
+    mbar_init(&ctl->mma_done, 1);
+    ctl->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (MODE != WS_LINEAR) wait_prerequisite_grids();   // counts and rows come from the kernels before
+  if (warp == 2) {
+    if constexpr (MODE == WS_LINEAR) {
+      if (lane == 0) {
+        ctl->tile_off[0] = ctl->row_off[0] = 0;
+        ctl->tile_off[1] = wm_tiles(p.M, NT);
+        ctl->row_off[1] = p.M;
+      }
+    } else {
+      wm_build_map(ctl->tile_off, ctl->row_off, p.counts, p.E, p.row_cap, NT);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0) allow_dependent_launch();
+  const uint32_t tmem = ctl->tmem_base;
+  volatile int* abort_flag = &ctl->abort_flag;
+
+  const int per_tile = MODE == WS_UP ? 64 : 128;      // output columns of 128 weight rows
+  const int row_tiles = (p.N + per_tile - 1) / per_tile;
+  const int units = ctl->tile_off[p.E] * p.splits * row_tiles;
+  const int steps = (p.K + 127) / 128;
+  const int groups = (p.K + p.w.group - 1) / p.w.group;
+  auto range = [&](const WmUnit& w, int& s0, int& s1) {   // steps of the unit
+    s0 = w.split * p.sps;
+    s1 = min(steps, s0 + p.sps);
+  };
+
+  if (warp < 4) {
+    if constexpr (NT == 128) regs_dec<WM_REGS_CTRL>();
+    if (warp == 0 && lane == 0) {
+      // ---------------- codes ----------------
+      const uint64_t pol = policy_evict_first();
+      uint32_t it = 0;
+      for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
+        const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
+        int s0, s1;
+        range(w, s0, s1);
+        const int y0 = MODE == WS_UP ? w.expert * 2 * p.N + w.rt * 64 : w.expert * p.N + w.rt * 128;
+        const int y1 = MODE == WS_UP ? y0 + p.N : y0 + 64;
+        for (int s = s0; s < s1; s += 2, ++it) {
+          const int st = it % S::CODE_STAGES;
+          if (!mbar_wait(&ctl->c_empty[st], ((it / S::CODE_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) break;
+          mbar_arrive_expect_tx(&ctl->c_full[st], WM_CODE_BYTES);
+          uint8_t* dst = ring_c + st * WM_CODE_BYTES;
+          tma_load_2d(dst, &code_map, s * 64, y0, &ctl->c_full[st], pol);
+          tma_load_2d(dst + WM_CODE_BYTES / 2, &code_map, s * 64, y1, &ctl->c_full[st], pol);
+        }
+      }
+      if (*abort_flag)
+        for (uint32_t i = 1; i <= S::CODE_STAGES && i <= it; ++i)
+          mbar_wait_drain(&ctl->c_full[(it - i) % S::CODE_STAGES], ((it - i) / S::CODE_STAGES) & 1u);
+    } else if (warp == 2 && lane == 0) {
+      // ---------------- token rows ----------------
+      if (MODE == WS_LINEAR) wait_prerequisite_grids();
+      const uint64_t pol = policy_evict_last();
+      uint32_t it = 0;
+      for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
+        const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
+        int s0, s1;
+        range(w, s0, s1);
+        const int boxes = (w.tokens + WM_BOX_TOK - 1) / WM_BOX_TOK;
+        const int b1 = min((p.K + 63) / 64, 2 * s1);
+        bool stop = false;
+        for (int b = 2 * s0; b < b1 && !stop; ++b)
+          for (int term = 0; term < TERMS; ++term, ++it) {
+            const int st = it % WM_B_STAGES;
+            if (!mbar_wait(&ctl->b_empty[st], ((it / WM_B_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) {
+              stop = true;
+              break;
+            }
+            mbar_arrive_expect_tx(&ctl->b_full[st], boxes * WM_BOX_TOK * 128);
+            for (int i = 0; i < boxes; ++i)
+              tma_load_2d(ring_b + st * S::B_BYTES + i * WM_BOX_TOK * 128, &x_map, b * 64,
+                          term * p.row_cap + w.row0 + i * WM_BOX_TOK, &ctl->b_full[st], pol);
+          }
+      }
+      if (*abort_flag)
+        for (uint32_t i = 1; i <= WM_B_STAGES && i <= it; ++i)
+          mbar_wait_drain(&ctl->b_full[(it - i) % WM_B_STAGES], ((it - i) / WM_B_STAGES) & 1u);
+    } else if (warp == 1 && lane == 0) {
+      // ---------------- mma ----------------
+      uint32_t b_it = 0, a_it = 0, d_it = 0;
+      bool stop = false;
+      const int per_block = p.w.group >= 64 ? 1 : 2;       // groups that start in a block of 64 columns
+      for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
+        const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
+        int s0, s1;
+        range(w, s0, s1);
+        const int n = (w.tokens + 15) & ~15;
+        constexpr uint32_t fmt = std::is_same_v<W, __half> ? 0u : (1u << 7) | (1u << 10);
+        const uint32_t idesc = (1u << 4) | fmt | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+        const int blocks = min((p.K + 63) / 64, 2 * s1) - 2 * s0;
+        uint32_t d = 0;
+        for (int b = 0; b < blocks && !stop; ++b) {
+          const uint32_t a_slot = a_it % WM_A_SLOTS;
+          if ((b & 1) == 0 && !mbar_wait_spin(&ctl->a_full[a_slot], (a_it / WM_A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA)) { stop = true; break; }
+          for (int term = 0; term < TERMS; ++term) {
+            const uint32_t e = b_it + term;
+            if (!mbar_wait_spin(&ctl->b_full[e % WM_B_STAGES], (e / WM_B_STAGES) & 1u, abort_flag, ST_TIMEOUT_MMA)) { stop = true; break; }
+          }
+          if (stop) break;
+          const uint32_t a = tmem + WM_A_COL + a_slot * 64 + (b & 1) * 32;
+          const bool opens = p.w.group < 128 || (b & 1) == 0;           // an accumulator starts with this block
+          const bool closes = p.w.group < 128 || (b & 1) || b + 1 == blocks;
+          for (int part = 0; part < per_block; ++part) {
+            const int k0 = (2 * s0 + b) * 64 + part * 32;
+            if (k0 >= p.K) break;
+            if (opens) {
+              const uint32_t q = d_it % S::BUFS;
+              if (!mbar_wait_spin(&ctl->d_empty[q], ((d_it / S::BUFS) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA)) { stop = true; break; }
+              d = tmem + q * NT;
+            }
+            tc_fence_after();
+            const int kk0 = part * 2, kk1 = per_block == 2 ? kk0 + 2 : 4;
+            for (int term = 0; term < TERMS; ++term) {
+              const uint32_t bb = smem_u32(ring_b + ((b_it + term) % WM_B_STAGES) * S::B_BYTES);
+              for (int kk = kk0; kk < kk1; ++kk)
+                tc_mma_ts(d, a + kk * 8, sdesc_k_sw128(bb + kk * 32), idesc,
+                          (opens && term == 0 && kk == kk0) ? 0u : 1u);
+            }
+            if (closes) {
+              tc_commit(&ctl->d_full[d_it % S::BUFS]);
+              ++d_it;
+            }
+          }
+          if (stop) break;
+          for (int term = 0; term < TERMS; ++term, ++b_it) tc_commit(&ctl->b_empty[b_it % WM_B_STAGES]);
+          if ((b & 1) || b + 1 == blocks) {
+            tc_commit(&ctl->a_empty[a_slot]);
+            ++a_it;
+          }
+        }
+      }
+      // Everything issued has finished before tensor and shared memory are given back.
+      tc_commit(&ctl->mma_done);
+      mbar_wait_drain(&ctl->mma_done, 0);
+    }
+  } else if (warp < 12) {
+    // ---------------- codes to numbers ----------------
+    if constexpr (NT == 128) regs_dec<WM_REGS_CONV>();
+    const int wg = (warp - 4) >> 2, q4 = warp & 3;
+    // Row of the shared tile behind this lane of tensor memory; `up` puts X1's 16 rows and X2's side by side.
+    const int srow = MODE == WS_UP ? (lane >> 4) * 64 + q4 * 16 + (lane & 15) : q4 * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    uint32_t c_it = 0, a_base = 0;
+    bool stop = false;
+    for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
+      const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
+      int s0, s1;
+      range(w, s0, s1);
+      const uint8_t* zrow = nullptr;
+      if (p.w.zero) {
+        const long long r = MODE == WS_UP
+            ? static_cast<long long>(w.expert) * 2 * p.N + (lane >> 4) * static_cast<long long>(p.N) + min(w.rt * 64 + q4 * 16 + (lane & 15), p.N - 1)
+            : static_cast<long long>(w.expert) * p.N + min(w.rt * 128 + srow, p.N - 1);
+        zrow = p.w.zero + r * groups;
+      }
+      for (int s = s0; s < s1; s += 2, ++c_it) {
+        const int mine = s + wg;
+        const bool valid = mine < s1;
+        uint32_t off[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          int z = 8;
+          if (zrow != nullptr && valid) z = __ldg(zrow + min((mine * 128 + i * 32) / p.w.group, groups - 1)) & 15;
+          off[i] = w4_offset<W>(z);
+        }
+        const int st = c_it % S::CODE_STAGES;
+        const uint32_t ph = (c_it / S::CODE_STAGES) & 1u;
+        if (!mbar_wait_warp(&ctl->c_full[st], ph, abort_flag, ST_TIMEOUT_EPILOGUE)) { stop = true; break; }
+        mbar_observe(&ctl->c_full[st], ph);
+        uint4 v[4];
+        const uint8_t* row = ring_c + st * WM_CODE_BYTES + srow * 128;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = *reinterpret_cast<const uint4*>(row + (((wg * 4 + c) ^ (srow & 7)) << 4));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->c_empty[st]);
+        if (!valid) continue;
+        const uint32_t a_it = a_base + static_cast<uint32_t>(mine - s0), slot = a_it % WM_A_SLOTS;
+        if (!mbar_wait_warp(&ctl->a_empty[slot], ((a_it / WM_A_SLOTS) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { stop = true; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t r[32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t o = off[hf * 2 + c];
+            const uint32_t word[4] = {v[hf * 2 + c].x, v[hf * 2 + c].y, v[hf * 2 + c].z, v[hf * 2 + c].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) r[c * 16 + i * 4 + j] = w4_pair<W>(word[i], j, o);
+          }
+          tmem_st32(tmem + lanes + WM_A_COL + slot * 64 + hf * 32, r);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->a_full[slot]);
+      }
+      a_base += static_cast<uint32_t>(s1 - s0);
+    }
+  } else {
+    // ---------------- scale and store ----------------
+    if constexpr (NT == 128) regs_inc<WM_REGS_EPI>();
+    const int q4 = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    uint32_t d_it = 0;
+    bool stop = false;
+    for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
+      const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
+      int s0, s1;
+      range(w, s0, s1);
+      const int g0 = s0 * 128 / p.w.group, g1 = min(groups, s1 * 128 / p.w.group);
+      const int col = MODE == WS_UP ? w.rt * 64 + q4 * 16 + (lane & 15) : w.rt * 128 + q4 * 32 + lane;
+      const long long mrow = MODE == WS_UP ? static_cast<long long>(w.expert) * 2 * p.N + (lane >> 4) * static_cast<long long>(p.N) + min(col, p.N - 1)
+                                           : static_cast<long long>(w.expert) * p.N + min(col, p.N - 1);
+      const T* srow = static_cast<const T*>(p.w.scale) + mrow * groups;
+      float total[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) total[i] = 0.0f;
+      float next = to_f32(srow[g0]);
+      for (int g = g0; g < g1; ++g, ++d_it) {
+        const float f = next;
+        if (g + 1 < g1) next = to_f32(srow[g + 1]);
+        const uint32_t q = d_it % S::BUFS, ph = (d_it / S::BUFS) & 1u;
+        if (!mbar_wait_warp(&ctl->d_full[q], ph, abort_flag, ST_TIMEOUT_EPILOGUE, true)) { stop = true; break; }
+        mbar_observe(&ctl->d_full[q], ph);
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < NT / 32; ++c)
+          if (c * 32 < w.tokens) {
+            float v[32];
+            tmem_ld32(tmem + lanes + q * NT + c * 32, v);
+            fma32_scaled(total + c * 32, v, f);
+          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->d_empty[q]);
+      }
+      if (stop) break;
+      if constexpr (MODE == WS_LINEAR) {
+        if (col < p.N) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            if (i < w.tokens) {
+              const long long at = static_cast<long long>(w.row0 + i) * p.N + col;
+              if (p.splits > 1)
+                p.y[static_cast<long long>(w.split) * p.M * p.N + at] = total[i];
+              else
+                static_cast<T*>(p.out)[at] = from_f32<T>(total[i]);
+            }
+        }
+      } else if constexpr (MODE == WS_DOWN) {
+        if (col < p.N) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            if (i < w.tokens) p.y[static_cast<long long>(w.row0 + i) * p.N + col] = total[i];
+        }
+      } else {
+        // Lanes 0-15 hold X1, lanes 16-31 X2 of the same columns: even tokens end in the first, odd in the second.
+        // hi + lo bf16 carry 16 bits of h; the columns go in pair order, zeros up to the next 8.
+        const int pos = pair_pos(col), mine = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < NT; i += 2)
+          if (i < w.tokens) {
+            const float give = mine ? total[i] : total[i + 1];
+            const float got = __shfl_xor_sync(0xffffffffu, give, 16);
+            const float u1 = mine ? got : total[i], u2 = mine ? total[i + 1] : got;
+            const float hv = col < p.N ? u1 * (u2 / (1.0f + expf(-u2))) : 0.0f;
+            if (i + mine < w.tokens && pos < p.h_pitch) {
+              const __nv_bfloat16 hi = __float2bfloat16_rn(hv);
+              const float rest = hv - __bfloat162float(hi);
+              const long long at = static_cast<long long>(w.row0 + i + mine) * p.h_pitch + pos;
+              p.h[at] = hi;
+              // An infinity or NaN has no remainder.
+              p.h[static_cast<long long>(p.row_cap) * p.h_pitch + at] = __float2bfloat16_rn(fabsf(rest) <= 3.4e38f ? rest : 0.0f);
+            }
+          }
+      }
+    }
+  }
+  if (MODE == WS_LINEAR) wait_prerequisite_grids();       // this grid ends after the one before it
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// ---- the kernels around it ----------------------------------------------------------------
+
+// 8 columns from k on (0 past K), in pair order.
+template <typename T>
+__device__ __forceinline__ uint4 ld_pairs(const T* row, int k, int K) {
+  alignas(16) T e[8];
+  if (k + 8 <= K && (reinterpret_cast<uintptr_t>(row + k) & 15u) == 0) {
+    *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(row + k));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = k + i < K ? row[k + i] : from_f32<T>(0.0f);
+  }
+  alignas(16) T o[8] = {e[0], e[4], e[1], e[5], e[2], e[6], e[3], e[7]};
+  return *reinterpret_cast<const uint4*>(o);
+}
+
+// Rows of x in pair order, columns padded with zeros to a multiple of 8.
+template <typename T>
+__global__ void __launch_bounds__(256) pair_rows_kernel(const T* x, long long x_stride, int M, int K, T* out) {
+  allow_dependent_launch();
+  const int per = (K + 7) / 8;
+  const long long n = static_cast<long long>(M) * per;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const long long m = i / per;
+    const int c = static_cast<int>(i % per);
+    reinterpret_cast<uint4*>(out)[i] = ld_pairs(x + m * x_stride, c * 8, K);
+  }
+}
+
+// Codes with a row pitch of a multiple of 16 bytes, for shapes whose own rows do not allow TMA.
+__global__ void __launch_bounds__(256) pad_codes_kernel(const uint8_t* codes, long long rows, int bytes, int pitch, uint8_t* out) {
+  const long long n = rows * (pitch / 4);
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const long long r = i / (pitch / 4);
+    const int o = static_cast<int>(i % (pitch / 4)) * 4;
+    uint32_t v = ld_u32_any(codes + r * bytes + o, bytes - o);
+    if (bytes - o < 4) v = bytes > o ? v & ((1u << (8 * (bytes - o))) - 1u) : 0u;
+    reinterpret_cast<uint32_t*>(out)[i] = v;
+  }
+}
+
+// Sum of the column parts of linear_w4, in order, rounded once.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* y, int splits, long long n, T* out) {
+  wait_prerequisite_grids();
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    float v = y[i];
+    for (int s = 1; s < splits; ++s) v += y[s * n + i];
+    out[i] = from_f32<T>(v);
+  }
+}
+
+// Each local pick takes a place in its expert's list. The order within a list changes from call to call and no
+// result with it: a row's products do not depend on the rows beside it.
+__global__ void __launch_bounds__(256) experts_slot_kernel(const int* idx, int n, int offset, int E, int* counts, int* slot) {
+  for (int r = blockIdx.x * 256 + threadIdx.x; r < n; r += gridDim.x * 256) {
+    const int id = idx[r];
+    const int e = id >= offset ? id - offset : -1;
+    slot[r] = e >= 0 && e < E ? atomicAdd(counts + e, 1) : -1;
+  }
+}
+
+// Copies each local pick's row to its expert's rows, in pair order; slot[r] becomes the row's place (or -1).
+template <typename T>
+__global__ void __launch_bounds__(256) experts_gather_kernel(const T* x, long long x_stride, const int* idx, int n, int k, int offset, int E,
+                                                             const int* counts, int H, int* slot, T* out) {
+  __shared__ int tile_off[RX_MAX_E + 1], row_off[RX_MAX_E + 1];
+  allow_dependent_launch();
+  if (threadIdx.x < 32) wm_build_map(tile_off, row_off, counts, E, n, 128);
+  __syncthreads();
+  const int per = (H + 7) / 8, lane = threadIdx.x & 31;
+  for (int r = (blockIdx.x * 256 + threadIdx.x) >> 5; r < n; r += gridDim.x * 8) {
+    const int s = slot[r];
+    if (s < 0) continue;
+    const int at = row_off[idx[r] - offset] + s;
+    if (at >= n) {
+      if (lane == 0) report_status(ST_BAD_INDEX);
+      continue;
+    }
+    const T* row = x + static_cast<long long>(r / k) * x_stride;
+    for (int c = lane; c < per; c += 32) reinterpret_cast<uint4*>(out)[static_cast<long long>(at) * per + c] = ld_pairs(row, c * 8, H);
+    __syncwarp();
+    if (lane == 0) slot[r] = at;
+  }
+}
+
+// out[t] = sum over the token's local picks, in their order, of weight * y[row], rounded once.
+template <typename T>
+__global__ void __launch_bounds__(256) experts_combine_kernel(const float* y, const int* place, const float* wt, int T_, int k, int H, T* out) {
+  wait_prerequisite_grids();
+  const long long n = static_cast<long long>(T_) * H;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const long long t = i / H;
+    const int c = static_cast<int>(i % H);
+    float acc = 0.0f;
+    for (int j = 0; j < k; ++j) {
+      const int r = place[t * k + j];
+      if (r >= 0) acc = fmaf(wt[t * k + j], y[static_cast<long long>(r) * H + c], acc);
+    }
+    out[i] = from_f32<T>(acc);
+  }
+}
+
+}  // namespace moe

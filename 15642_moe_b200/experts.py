@@ -163,8 +163,13 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: t
         _check(out.dtype == x.dtype and out.shape == (M, N) and out.is_contiguous() and out.device == dev,
                "out must be a contiguous [M, N] tensor of x's type on its device")
     if M:
-        _call(_native.cuda_lib().moe_linear_w4, dev, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), codes.data_ptr(),
-              scale.data_ptr(), None if zero is None else zero.data_ptr(), group, M, N, K, out.data_ptr())
+        lib, ws, need = _native.cuda_lib(), None, 0
+        if M > 8:
+            need = int(lib.moe_linear_w4_workspace_bytes(M, N, K))
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _call(lib.moe_linear_w4, dev, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), codes.data_ptr(), scale.data_ptr(),
+              None if zero is None else zero.data_ptr(), group, M, N, K, out.data_ptr(),
+              None if ws is None else ws.data_ptr(), need)
     return out
 
 
