@@ -775,10 +775,10 @@ int wm_prepare(int smem, bool split_regs) {
 }
 
 template <typename T, int MODE, int NT>
-int launch_w4_mma_nt(DeviceInfo* d, const CUtensorMap& cm, const CUtensorMap& xm, const WmArgs& a, long long units, cudaStream_t st) {
+int launch_w4_mma_nt(DeviceInfo* d, const CUtensorMap& cm, const CUtensorMap& xm, const CUtensorMap& xf, const WmArgs& a, long long units, cudaStream_t st) {
   if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT>>(WM_SMEM<NT>, NT == 128)) return rc;
   const int grid = units < d->num_sms ? static_cast<int>(units) : d->num_sms;
-  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT>, grid < 1 ? 1 : grid, WM_THREADS, WM_SMEM<NT>, st, cm, xm, a),
+  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT>, grid < 1 ? 1 : grid, WM_THREADS, WM_SMEM<NT>, st, cm, xm, xf, a),
                     "w4_mma launch");
 }
 
@@ -787,10 +787,11 @@ template <typename T, int MODE>
 int launch_w4_mma(DeviceInfo* d, const WmArgs& a, const void* x, long long x_rows, int tile, cudaStream_t st) {
   const int pitch = round_up(w4_bytes(a.K), 16), width = round_up(a.K, 8);
   const long long rows = static_cast<long long>(a.E) * (MODE == WS_UP ? 2 : 1) * a.N;
-  CUtensorMap cm, xm;
+  CUtensorMap cm, xm, xf;
   if (int rc = w4_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w.codes, pitch, rows, pitch, 128, 64, &cm)) return rc;
   const CUtensorMapDataType t = MODE != WS_DOWN && std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, WM_BOX_TOK, &xm)) return rc;
+  if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, tile, &xf)) return rc;
   const int per = MODE == WS_UP ? 64 : 128;
   // Most units that there can be: every expert's tokens in tiles, or one token in each.
   const long long row_tiles = (static_cast<long long>(a.N) + per - 1) / per;
@@ -798,9 +799,9 @@ int launch_w4_mma(DeviceInfo* d, const WmArgs& a, const void* x, long long x_row
   const long long tiles = MODE == WS_LINEAR ? (tokens + tile - 1) / tile : (tokens < a.E ? tokens : a.E) + tokens / tile;
   const long long units = tiles * row_tiles * a.splits;
   switch (tile) {
-    case 32: return launch_w4_mma_nt<T, MODE, 32>(d, cm, xm, a, units, st);
-    case 64: return launch_w4_mma_nt<T, MODE, 64>(d, cm, xm, a, units, st);
-    default: return launch_w4_mma_nt<T, MODE, 128>(d, cm, xm, a, units, st);
+    case 32: return launch_w4_mma_nt<T, MODE, 32>(d, cm, xm, xf, a, units, st);
+    case 64: return launch_w4_mma_nt<T, MODE, 64>(d, cm, xm, xf, a, units, st);
+    default: return launch_w4_mma_nt<T, MODE, 128>(d, cm, xm, xf, a, units, st);
   }
 }
 

@@ -86,13 +86,22 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // D(tmem) (+)= A(tmem, 128 x 16) x B(smem desc)^T, bf16 or f16 operands (idesc), fp32 accumulate.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Only where `issue` is set.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t issue) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(issue)
       : "memory");
+}
+
+// Warp-wide bounded wait by polling: every lane sees the phase complete, and all agree on giving up.
+__device__ __forceinline__ bool wait_mma(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, abort_flag, ST_TIMEOUT_MMA));
 }
 
 // Tiles of up to NT tokens: an expert's rows in equal parts.
@@ -170,7 +179,7 @@ __device__ __forceinline__ WmUnit wm_unit(const WmCtrl* ctl, const WmArgs& p, in
 template <typename T, int MODE, int NT>
 __global__ void __launch_bounds__(WM_THREADS, 1)
     w4_mma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map,
-                  const __grid_constant__ WmArgs p) {
+                  const __grid_constant__ CUtensorMap x_map_full, const __grid_constant__ WmArgs p) {
   using W = typename std::conditional<MODE == WS_DOWN, __nv_bfloat16, T>::type;   // the operands' type
   using S = WmShape<NT>;
   constexpr int TERMS = MODE == WS_DOWN ? 2 : 1;
@@ -268,6 +277,8 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
         int s0, s1;
         range(w, s0, s1);
+        // Few tokens: boxes of 16 rows; more than half a tile: one box (rows past the tile's are read for nothing).
+        const bool full = 2 * w.tokens > NT;
         const int boxes = (w.tokens + WM_BOX_TOK - 1) / WM_BOX_TOK;
         const int b1 = min((p.K + 63) / 64, 2 * s1);
         bool stop = false;
@@ -278,7 +289,10 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
               stop = true;
               break;
             }
-            mbar_arrive_expect_tx(&ctl->b_full[st], boxes * WM_BOX_TOK * 128);
+            mbar_arrive_expect_tx(&ctl->b_full[st], full ? S::B_BYTES : boxes * WM_BOX_TOK * 128);
+            if (full)
+              tma_load_2d(ring_b + st * S::B_BYTES, &x_map_full, b * 64, term * p.row_cap + w.row0, &ctl->b_full[st], pol);
+            else
             for (int i = 0; i < boxes; ++i)
               tma_load_2d(ring_b + st * S::B_BYTES + i * WM_BOX_TOK * 128, &x_map, b * 64,
                           term * p.row_cap + w.row0 + i * WM_BOX_TOK, &ctl->b_full[st], pol);
@@ -287,12 +301,13 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       if (*abort_flag)
         for (uint32_t i = 1; i <= WM_B_STAGES && i <= it; ++i)
           mbar_wait_drain(&ctl->b_full[(it - i) % WM_B_STAGES], ((it - i) / WM_B_STAGES) & 1u);
-    } else if (warp == 1 && lane == 0) {
-      // ---------------- mma ----------------
+    } else if (warp == 1) {
+      // ---------------- mma: the warp runs together, one lane issues ----------------
+      const uint32_t leader = lane == 0 ? 1u : 0u;
+      const uint64_t b_desc0 = sdesc_k_sw128(smem_u32(ring_b));
       uint32_t b_it = 0, a_it = 0, d_it = 0;
-      bool stop = false;
-      const int per_block = p.w.group >= 64 ? 1 : 2;       // groups that start in a block of 64 columns
-      for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
         const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
         int s0, s1;
         range(w, s0, s1);
@@ -300,50 +315,75 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         constexpr uint32_t fmt = std::is_same_v<W, __half> ? 0u : (1u << 7) | (1u << 10);
         const uint32_t idesc = (1u << 4) | fmt | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
         const int blocks = min((p.K + 63) / 64, 2 * s1) - 2 * s0;
-        uint32_t d = 0;
-        for (int b = 0; b < blocks && !stop; ++b) {
-          const uint32_t a_slot = a_it % WM_A_SLOTS;
-          if ((b & 1) == 0 && !mbar_wait_spin(&ctl->a_full[a_slot], (a_it / WM_A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA)) { stop = true; break; }
+        // One block of 64 columns; LAST: the last of its step. An accumulator covers one block (group 64), the two
+        // of a step (128) or half a block (32).
+        auto block = [&](int b, uint32_t a, bool first, bool last) {
+#pragma unroll
           for (int term = 0; term < TERMS; ++term) {
             const uint32_t e = b_it + term;
-            if (!mbar_wait_spin(&ctl->b_full[e % WM_B_STAGES], (e / WM_B_STAGES) & 1u, abort_flag, ST_TIMEOUT_MMA)) { stop = true; break; }
+            ok = ok && wait_mma(&ctl->b_full[e % WM_B_STAGES], (e / WM_B_STAGES) & 1u, abort_flag);
           }
-          if (stop) break;
-          const uint32_t a = tmem + WM_A_COL + a_slot * 64 + (b & 1) * 32;
-          const bool opens = p.w.group < 128 || (b & 1) == 0;           // an accumulator starts with this block
-          const bool closes = p.w.group < 128 || (b & 1) || b + 1 == blocks;
-          for (int part = 0; part < per_block; ++part) {
-            const int k0 = (2 * s0 + b) * 64 + part * 32;
-            if (k0 >= p.K) break;
-            if (opens) {
-              const uint32_t q = d_it % S::BUFS;
-              if (!mbar_wait_spin(&ctl->d_empty[q], ((d_it / S::BUFS) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA)) { stop = true; break; }
-              d = tmem + q * NT;
-            }
+          auto open = [&]() {
+            const uint32_t q = d_it % S::BUFS;
+            ok = ok && wait_mma(&ctl->d_empty[q], ((d_it / S::BUFS) & 1u) ^ 1u, abort_flag);
+          };
+          auto close = [&]() {
+            if (leader) tc_commit(&ctl->d_full[d_it % S::BUFS]);
+            ++d_it;
+          };
+          if (p.w.group >= 64) {
+            const bool opens = first || p.w.group == 64;
+            if (opens) open();
+            if (!ok) return;
             tc_fence_after();
-            const int kk0 = part * 2, kk1 = per_block == 2 ? kk0 + 2 : 4;
+            const uint32_t d = tmem + (d_it % S::BUFS) * NT;
+#pragma unroll
             for (int term = 0; term < TERMS; ++term) {
-              const uint32_t bb = smem_u32(ring_b + ((b_it + term) % WM_B_STAGES) * S::B_BYTES);
-              for (int kk = kk0; kk < kk1; ++kk)
-                tc_mma_ts(d, a + kk * 8, sdesc_k_sw128(bb + kk * 32), idesc,
-                          (opens && term == 0 && kk == kk0) ? 0u : 1u);
+              const uint64_t bd = b_desc0 + ((b_it + term) % WM_B_STAGES) * (S::B_BYTES >> 4);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, opens && term == 0 && kk == 0 ? 0u : 1u, leader);
             }
-            if (closes) {
-              tc_commit(&ctl->d_full[d_it % S::BUFS]);
-              ++d_it;
+            if (last || p.w.group == 64) close();
+          } else {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              if ((2 * s0 + b) * 64 + part * 32 < p.K) {
+                open();
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t d = tmem + (d_it % S::BUFS) * NT;
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) {
+                  const uint64_t bd = b_desc0 + ((b_it + term) % WM_B_STAGES) * (S::B_BYTES >> 4);
+#pragma unroll
+                  for (int kk = 2 * part; kk < 2 * part + 2; ++kk)
+                    tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, term == 0 && kk == 2 * part ? 0u : 1u, leader);
+                }
+                close();
+              }
             }
           }
-          if (stop) break;
-          for (int term = 0; term < TERMS; ++term, ++b_it) tc_commit(&ctl->b_empty[b_it % WM_B_STAGES]);
-          if ((b & 1) || b + 1 == blocks) {
-            tc_commit(&ctl->a_empty[a_slot]);
-            ++a_it;
-          }
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term, ++b_it)
+            if (leader) tc_commit(&ctl->b_empty[b_it % WM_B_STAGES]);
+        };
+        for (int b = 0; b < blocks && ok; b += 2, ++a_it) {
+          const uint32_t slot = a_it % WM_A_SLOTS;
+          ok = wait_mma(&ctl->a_full[slot], (a_it / WM_A_SLOTS) & 1u, abort_flag);
+          if (!ok) break;
+          const uint32_t a = tmem + WM_A_COL + slot * 64;
+          block(b, a, true, b + 1 == blocks);
+          if (ok && b + 1 < blocks) block(b + 1, a + 32, false, true);
+          if (ok && leader) tc_commit(&ctl->a_empty[slot]);
         }
       }
       // Everything issued has finished before tensor and shared memory are given back.
-      tc_commit(&ctl->mma_done);
-      mbar_wait_drain(&ctl->mma_done, 0);
+      if (leader) {
+        tc_commit(&ctl->mma_done);
+        mbar_wait_drain(&ctl->mma_done, 0);
+      }
+      __syncwarp();
     }
   } else if (warp < 12) {
     // ---------------- codes to numbers ----------------
