@@ -86,22 +86,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // D(tmem) (+)= A(tmem, 128 x 16) x B(smem desc)^T, bf16 or f16 operands (idesc), fp32 accumulate.
-// Only where `issue` is set.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate,
-                                          uint32_t issue) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(issue)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
-// Warp-wide bounded wait by polling: every lane sees the phase complete, and all agree on giving up.
-__device__ __forceinline__ bool wait_mma(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
-  return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, abort_flag, ST_TIMEOUT_MMA));
+// One lane of a converged warp. The compiler then knows that a single thread runs what follows and keeps the operands of
+// mma and copy instructions in uniform registers: an mma with 16 tokens issues every 9 cycles, behind `lane == 0` every 46.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 // Tiles of up to NT tokens: an expert's rows in equal parts.
@@ -246,7 +249,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
 
   if (warp < 4) {
     if constexpr (NT == 128) regs_dec<WM_REGS_CTRL>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       // ---------------- codes ----------------
       const uint64_t pol = policy_evict_first();
       uint32_t it = 0;
@@ -268,7 +271,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       if (*abort_flag)
         for (uint32_t i = 1; i <= S::CODE_STAGES && i <= it; ++i)
           mbar_wait_drain(&ctl->c_full[(it - i) % S::CODE_STAGES], ((it - i) / S::CODE_STAGES) & 1u);
-    } else if (warp == 2 && lane == 0) {
+    } else if (warp == 2 && elect_one()) {
       // ---------------- token rows ----------------
       if (MODE == WS_LINEAR) wait_prerequisite_grids();
       const uint64_t pol = policy_evict_last();
@@ -301,9 +304,8 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       if (*abort_flag)
         for (uint32_t i = 1; i <= WM_B_STAGES && i <= it; ++i)
           mbar_wait_drain(&ctl->b_full[(it - i) % WM_B_STAGES], ((it - i) / WM_B_STAGES) & 1u);
-    } else if (warp == 1) {
-      // ---------------- mma: the warp runs together, one lane issues ----------------
-      const uint32_t leader = lane == 0 ? 1u : 0u;
+    } else if (warp == 1 && elect_one()) {
+      // ---------------- mma ----------------
       const uint64_t b_desc0 = sdesc_k_sw128(smem_u32(ring_b));
       uint32_t b_it = 0, a_it = 0, d_it = 0;
       bool ok = true;
@@ -321,14 +323,14 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
 #pragma unroll
           for (int term = 0; term < TERMS; ++term) {
             const uint32_t e = b_it + term;
-            ok = ok && wait_mma(&ctl->b_full[e % WM_B_STAGES], (e / WM_B_STAGES) & 1u, abort_flag);
+            ok = ok && mbar_wait_spin(&ctl->b_full[e % WM_B_STAGES], (e / WM_B_STAGES) & 1u, abort_flag, ST_TIMEOUT_MMA);
           }
           auto open = [&]() {
             const uint32_t q = d_it % S::BUFS;
-            ok = ok && wait_mma(&ctl->d_empty[q], ((d_it / S::BUFS) & 1u) ^ 1u, abort_flag);
+            ok = ok && mbar_wait_spin(&ctl->d_empty[q], ((d_it / S::BUFS) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA);
           };
           auto close = [&]() {
-            if (leader) tc_commit(&ctl->d_full[d_it % S::BUFS]);
+            tc_commit(&ctl->d_full[d_it % S::BUFS]);
             ++d_it;
           };
           if (p.w.group >= 64) {
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
               const uint64_t bd = b_desc0 + ((b_it + term) % WM_B_STAGES) * (S::B_BYTES >> 4);
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
-                tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, opens && term == 0 && kk == 0 ? 0u : 1u, leader);
+                tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, opens && term == 0 && kk == 0 ? 0u : 1u);
             }
             if (last || p.w.group == 64) close();
           } else {
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
                   const uint64_t bd = b_desc0 + ((b_it + term) % WM_B_STAGES) * (S::B_BYTES >> 4);
 #pragma unroll
                   for (int kk = 2 * part; kk < 2 * part + 2; ++kk)
-                    tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, term == 0 && kk == 2 * part ? 0u : 1u, leader);
+                    tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, term == 0 && kk == 2 * part ? 0u : 1u);
                 }
                 close();
               }
@@ -366,24 +368,21 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
           }
 #pragma unroll
           for (int term = 0; term < TERMS; ++term, ++b_it)
-            if (leader) tc_commit(&ctl->b_empty[b_it % WM_B_STAGES]);
+            tc_commit(&ctl->b_empty[b_it % WM_B_STAGES]);
         };
         for (int b = 0; b < blocks && ok; b += 2, ++a_it) {
           const uint32_t slot = a_it % WM_A_SLOTS;
-          ok = wait_mma(&ctl->a_full[slot], (a_it / WM_A_SLOTS) & 1u, abort_flag);
+          ok = mbar_wait_spin(&ctl->a_full[slot], (a_it / WM_A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA);
           if (!ok) break;
           const uint32_t a = tmem + WM_A_COL + slot * 64;
           block(b, a, true, b + 1 == blocks);
           if (ok && b + 1 < blocks) block(b + 1, a + 32, false, true);
-          if (ok && leader) tc_commit(&ctl->a_empty[slot]);
+          if (ok) tc_commit(&ctl->a_empty[slot]);
         }
       }
       // Everything issued has finished before tensor and shared memory are given back.
-      if (leader) {
-        tc_commit(&ctl->mma_done);
-        mbar_wait_drain(&ctl->mma_done, 0);
-      }
-      __syncwarp();
+      tc_commit(&ctl->mma_done);
+      mbar_wait_drain(&ctl->mma_done, 0);
     }
   } else if (warp < 12) {
     // ---------------- codes to numbers ----------------
