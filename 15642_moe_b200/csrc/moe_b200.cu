@@ -679,12 +679,12 @@ int wm_tile(long long rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 constexpr int WM_SMS = 148;   // the split rule's SM count: results and workspace sizes do not depend on the device
 
-// linear_w4: parts of the columns, so that few row tiles still fill the SMs; four steps of 128 each at least.
+// linear_w4: parts of the columns, so that few row tiles still fill the SMs; two steps each at least.
 int wm_splits(int M, int N, int K) {
   const long long nt = wm_tile(M), units = (M + nt - 1) / nt * ((N + 127ll) / 128);
-  const int steps = (K + 127) / 128;
+  const int steps = (K + WM_STEP - 1) / WM_STEP;
   long long s = WM_SMS / units;
-  if (s > steps / 4) s = steps / 4;
+  if (s > steps / 2) s = steps / 2;
   if (s > 16) s = 16;
   return s < 1 ? 1 : static_cast<int>(s);
 }
@@ -774,35 +774,45 @@ int wm_prepare(int smem, bool split_regs) {
   return MOE_OK;
 }
 
-template <typename T, int MODE, int NT>
-int launch_w4_mma_nt(DeviceInfo* d, const CUtensorMap& cm, const CUtensorMap& xm, const CUtensorMap& xf, const WmArgs& a, long long units, cudaStream_t st) {
-  if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT>>(WM_SMEM<NT>, NT == 128)) return rc;
+template <typename T, int MODE, int NT, int G>
+int launch_w4_mma_g(DeviceInfo* d, const CUtensorMap& cm, const CUtensorMap& xm, const CUtensorMap& xf, const WmArgs& a, long long units,
+                    cudaStream_t st) {
+  constexpr int smem = WM_SMEM<NT, MODE == WS_DOWN ? 2 : 1>;
+  if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT, G>>(smem, NT == 128)) return rc;
   const int grid = units < d->num_sms ? static_cast<int>(units) : d->num_sms;
-  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT>, grid < 1 ? 1 : grid, WM_THREADS, WM_SMEM<NT>, st, cm, xm, xf, a),
+  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT, G>, grid < 1 ? 1 : grid, WM_THREADS, smem, st, cm, xm, xf, a),
                     "w4_mma launch");
 }
 
-// `rows`: tokens (routes) in the x buffer, each `width` columns; tile: expected tokens of one expert.
-template <typename T, int MODE>
-int launch_w4_mma(DeviceInfo* d, const WmArgs& a, const void* x, long long x_rows, int tile, cudaStream_t st) {
+// x_rows: rows of the token buffer; tile: tokens per tile.
+template <typename T, int MODE, int NT>
+int launch_w4_mma_nt(DeviceInfo* d, const WmArgs& a, const void* x, long long x_rows, cudaStream_t st) {
   const int pitch = round_up(w4_bytes(a.K), 16), width = round_up(a.K, 8);
   const long long rows = static_cast<long long>(a.E) * (MODE == WS_UP ? 2 : 1) * a.N;
   CUtensorMap cm, xm, xf;
   if (int rc = w4_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w.codes, pitch, rows, pitch, 128, 64, &cm)) return rc;
   const CUtensorMapDataType t = MODE != WS_DOWN && std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, WM_BOX_TOK, &xm)) return rc;
-  if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, tile, &xf)) return rc;
+  if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, NT, &xf)) return rc;
   const int per = MODE == WS_UP ? 64 : 128;
   // Most units that there can be: every expert's tokens in tiles, or one token in each.
   const long long row_tiles = (static_cast<long long>(a.N) + per - 1) / per;
   const long long tokens = MODE == WS_LINEAR ? a.M : a.row_cap;
-  const long long tiles = MODE == WS_LINEAR ? (tokens + tile - 1) / tile : (tokens < a.E ? tokens : a.E) + tokens / tile;
+  const long long tiles = MODE == WS_LINEAR ? (tokens + NT - 1) / NT : (tokens < a.E ? tokens : a.E) + tokens / NT;
   const long long units = tiles * row_tiles * a.splits;
-  switch (tile) {
-    case 32: return launch_w4_mma_nt<T, MODE, 32>(d, cm, xm, xf, a, units, st);
-    case 64: return launch_w4_mma_nt<T, MODE, 64>(d, cm, xm, xf, a, units, st);
-    default: return launch_w4_mma_nt<T, MODE, 128>(d, cm, xm, xf, a, units, st);
+  switch (a.w.group) {
+    case 32: return launch_w4_mma_g<T, MODE, NT, 32>(d, cm, xm, xf, a, units, st);
+    case 64: return launch_w4_mma_g<T, MODE, NT, 64>(d, cm, xm, xf, a, units, st);
+    default: return launch_w4_mma_g<T, MODE, NT, 128>(d, cm, xm, xf, a, units, st);
   }
+}
+
+template <typename T, int MODE>
+int launch_w4_mma(DeviceInfo* d, const WmArgs& a, const void* x, long long x_rows, int tile, cudaStream_t st) {
+  if (tile == 32) return launch_w4_mma_nt<T, MODE, 32>(d, a, x, x_rows, st);
+  // The experts' second product has two terms per token: 64 tokens fill its ring.
+  if constexpr (MODE == WS_DOWN) return launch_w4_mma_nt<T, MODE, 64>(d, a, x, x_rows, st);
+  else return tile == 64 ? launch_w4_mma_nt<T, MODE, 64>(d, a, x, x_rows, st) : launch_w4_mma_nt<T, MODE, 128>(d, a, x, x_rows, st);
 }
 
 // Codes as TMA can read them: the caller's, or a copy with padded rows.
@@ -842,8 +852,9 @@ int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Mat
   a.M = M;
   a.row_cap = M;
   a.splits = wm_splits(M, N, K);
-  a.sps = round_up((static_cast<long long>((K + 127) / 128) + a.splits - 1) / a.splits, 2);
-  a.splits = ((K + 127) / 128 + a.sps - 1) / a.sps;
+  const int steps = (K + WM_STEP - 1) / WM_STEP;
+  a.sps = (steps + a.splits - 1) / a.splits;
+  a.splits = (steps + a.sps - 1) / a.sps;
   a.y = reinterpret_cast<float*>(W + ws.parts);
   a.out = out;
   if (int rc = launch_w4_mma<T, WS_LINEAR>(d, a, W + ws.x, M, wm_tile(M), st)) return rc;
@@ -901,8 +912,8 @@ int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W
   up.splits = down.splits = 1;
   up.N = down.K = p.I;
   up.K = down.N = p.H;
-  up.sps = round_up((up.K + 127) / 128, 2);
-  down.sps = round_up((down.K + 127) / 128, 2);
+  up.sps = (up.K + WM_STEP - 1) / WM_STEP;
+  down.sps = (down.K + WM_STEP - 1) / WM_STEP;
   up.h = h;
   up.h_pitch = round_up(p.I, 8);
   down.y = y;

@@ -23,38 +23,41 @@
 namespace moe {
 
 constexpr int WM_THREADS = 512;
-constexpr int WM_CODE_BYTES = 128 * 128;        // 128 rows x 256 columns
-constexpr int WM_B_STAGES = 8;                  // 64 columns of the tile's tokens each
-constexpr int WM_A_SLOTS = 4;                   // steps of 128 columns in tensor memory (64 of its columns each)
+constexpr int WM_STEP = 256;                    // columns per step
+constexpr int WM_CODE_BYTES = 128 * WM_STEP / 2;
+constexpr int WM_A_SLOTS = 2;                   // steps in tensor memory (128 of its columns each), one per warpgroup
 constexpr int WM_A_COL = 256;                   // accumulators in [0, 256), weights in [256, 512)
-constexpr int WM_MAX_BUFS = 4;
-constexpr int WM_BOX_TOK = 16;                  // token rows per TMA box
+constexpr int WM_D_COLS = 128;                  // columns of one batch of accumulators, two batches
+constexpr int WM_BOX_TOK = 16;                  // token rows per small TMA box
 constexpr int WM_REGS_CTRL = 48, WM_REGS_CONV = 104, WM_REGS_EPI = 232;   // register split for NT = 128
 constexpr int WM_LAUNCH_REGS_MIN = (WM_REGS_CTRL + 2 * WM_REGS_CONV + WM_REGS_EPI + 3) / 4;
 
-template <int NT>
+// Shared memory: a ring of steps of codes, a ring of token rows. An entry of the second holds B_COLS columns of every
+// term (up to 64 KB), so that a step of few tokens is one entry.
+template <int NT, int TERMS>
 struct WmShape {
-  static constexpr int CODE_STAGES = NT == 128 ? 5 : 8;
-  static constexpr int B_BYTES = NT * 128;
-  static constexpr int BUFS = 256 / NT < WM_MAX_BUFS ? 256 / NT : WM_MAX_BUFS;   // accumulators
-  static constexpr int RING = CODE_STAGES * WM_CODE_BYTES + WM_B_STAGES * B_BYTES;
+  static constexpr int B_COLS = NT * TERMS >= 128 ? 128 : 256;
+  static constexpr int B_BYTES = NT * TERMS * B_COLS * 2;
+  static constexpr int B_STAGES = 4;
+  static constexpr int CODE_STAGES = B_BYTES >= 32768 ? 5 : 8;
+  static constexpr int RING = CODE_STAGES * WM_CODE_BYTES + B_STAGES * B_BYTES;
+  static_assert(RING <= 212992, "rings too large");
 };
 
 struct WmCtrl {
   uint64_t c_full[8], c_empty[8];
-  uint64_t b_full[WM_B_STAGES], b_empty[WM_B_STAGES];
+  uint64_t b_full[4], b_empty[4];
   uint64_t a_full[WM_A_SLOTS], a_empty[WM_A_SLOTS];
-  uint64_t d_full[WM_MAX_BUFS], d_empty[WM_MAX_BUFS];
+  uint64_t d_full[2], d_empty[2];
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort_flag;
-  int tiles, rows;                              // token tiles of all experts; routes
   int tile_off[RX_MAX_E + 1];                   // first token tile of each expert
   int row_off[RX_MAX_E + 1];                    // first row of each expert in the route-ordered buffers
 };
 
-template <int NT>
-constexpr int WM_SMEM = WmShape<NT>::RING + static_cast<int>(sizeof(WmCtrl)) + 1024;
+template <int NT, int TERMS>
+constexpr int WM_SMEM = WmShape<NT, TERMS>::RING + static_cast<int>(sizeof(WmCtrl)) + 1024;
 
 struct WmArgs {
   W4Matrix w;
@@ -62,7 +65,7 @@ struct WmArgs {
   int M;                    // linear: tokens
   const int* counts;        // [E] routes per expert (up, down)
   int row_cap;              // rows of the route-ordered buffers
-  int splits, sps;          // linear: parts of the columns, each of `sps` (even) steps of 128
+  int splits, sps;          // linear: parts of the columns, each of `sps` steps
   __nv_bfloat16* h;         // up: [2][row_cap][Ip] hi and lo of the intermediate, columns in pair order
   int h_pitch;              // Ip
   float* y;                 // down: [row_cap][N]; linear with splits: [splits][M][N]
@@ -105,6 +108,12 @@ __device__ __forceinline__ bool elect_one() {
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(p));
   return p != 0;
+}
+
+// Bounded wait by polling, all lanes of a converged warp; they agree on giving up.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int who) {
+  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, abort_flag, who));
 }
 
 // Tiles of up to NT tokens: an expert's rows in equal parts.
@@ -179,13 +188,17 @@ __device__ __forceinline__ WmUnit wm_unit(const WmCtrl* ctl, const WmArgs& p, in
   return w;
 }
 
-template <typename T, int MODE, int NT>
+template <typename T, int MODE, int NT, int G>
 __global__ void __launch_bounds__(WM_THREADS, 1)
     w4_mma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map,
                   const __grid_constant__ CUtensorMap x_map_full, const __grid_constant__ WmArgs p) {
   using W = typename std::conditional<MODE == WS_DOWN, __nv_bfloat16, T>::type;   // the operands' type
-  using S = WmShape<NT>;
   constexpr int TERMS = MODE == WS_DOWN ? 2 : 1;
+  using S = WmShape<NT, TERMS>;
+  constexpr int GPS = WM_STEP / G;                                      // groups per step
+  constexpr int GPB = WM_D_COLS / NT < GPS ? WM_D_COLS / NT : GPS;      // groups per batch of accumulators
+  constexpr int BATCHES = GPS / GPB;                                    // batches per step
+  constexpr int ENTRIES = WM_STEP / S::B_COLS;                          // entries of token rows per step
   extern __shared__ uint8_t wm_raw[];
   uint8_t* smem = align_1024(wm_raw);
   uint8_t* ring_c = smem;
@@ -196,9 +209,9 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::CODE_STAGES; ++i) {
       mbar_init(&ctl->c_full[i], 1);
-      mbar_init(&ctl->c_empty[i], 8);
+      mbar_init(&ctl->c_empty[i], 4);
     }
-    for (int i = 0; i < WM_B_STAGES; ++i) {
+    for (int i = 0; i < S::B_STAGES; ++i) {
       mbar_init(&ctl->b_full[i], 1);
       mbar_init(&ctl->b_empty[i], 1);
     }
@@ -206,7 +219,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       mbar_init(&ctl->a_full[i], 4);
       mbar_init(&ctl->a_empty[i], 1);
     }
-    for (int i = 0; i < S::BUFS; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->d_full[i], 1);
       mbar_init(&ctl->d_empty[i], 4);
     }
@@ -240,8 +253,8 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
   const int per_tile = MODE == WS_UP ? 64 : 128;      // output columns of 128 weight rows
   const int row_tiles = (p.N + per_tile - 1) / per_tile;
   const int units = ctl->tile_off[p.E] * p.splits * row_tiles;
-  const int steps = (p.K + 127) / 128;
-  const int groups = (p.K + p.w.group - 1) / p.w.group;
+  const int steps = (p.K + WM_STEP - 1) / WM_STEP;
+  const int groups = (p.K + G - 1) / G;
   auto range = [&](const WmUnit& w, int& s0, int& s1) {   // steps of the unit
     s0 = w.split * p.sps;
     s1 = min(steps, s0 + p.sps);
@@ -259,13 +272,13 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         range(w, s0, s1);
         const int y0 = MODE == WS_UP ? w.expert * 2 * p.N + w.rt * 64 : w.expert * p.N + w.rt * 128;
         const int y1 = MODE == WS_UP ? y0 + p.N : y0 + 64;
-        for (int s = s0; s < s1; s += 2, ++it) {
+        for (int s = s0; s < s1; ++s, ++it) {
           const int st = it % S::CODE_STAGES;
           if (!mbar_wait(&ctl->c_empty[st], ((it / S::CODE_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) break;
           mbar_arrive_expect_tx(&ctl->c_full[st], WM_CODE_BYTES);
           uint8_t* dst = ring_c + st * WM_CODE_BYTES;
-          tma_load_2d(dst, &code_map, s * 64, y0, &ctl->c_full[st], pol);
-          tma_load_2d(dst + WM_CODE_BYTES / 2, &code_map, s * 64, y1, &ctl->c_full[st], pol);
+          tma_load_2d(dst, &code_map, s * (WM_STEP / 2), y0, &ctl->c_full[st], pol);
+          tma_load_2d(dst + WM_CODE_BYTES / 2, &code_map, s * (WM_STEP / 2), y1, &ctl->c_full[st], pol);
         }
       }
       if (*abort_flag)
@@ -283,27 +296,28 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         // Few tokens: boxes of 16 rows; more than half a tile: one box (rows past the tile's are read for nothing).
         const bool full = 2 * w.tokens > NT;
         const int boxes = (w.tokens + WM_BOX_TOK - 1) / WM_BOX_TOK;
-        const int b1 = min((p.K + 63) / 64, 2 * s1);
-        bool stop = false;
-        for (int b = 2 * s0; b < b1 && !stop; ++b)
-          for (int term = 0; term < TERMS; ++term, ++it) {
-            const int st = it % WM_B_STAGES;
-            if (!mbar_wait(&ctl->b_empty[st], ((it / WM_B_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) {
-              stop = true;
-              break;
+        const uint32_t bytes = (full ? NT : boxes * WM_BOX_TOK) * S::B_COLS * 2 * TERMS;
+        for (int c = s0 * ENTRIES; c < s1 * ENTRIES; ++c, ++it) {
+          const int st = it % S::B_STAGES;
+          if (!mbar_wait(&ctl->b_empty[st], ((it / S::B_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) break;
+          mbar_arrive_expect_tx(&ctl->b_full[st], bytes);
+          uint8_t* dst = ring_b + st * S::B_BYTES;
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+            for (int q = 0; q < S::B_COLS / 64; ++q, dst += NT * 128) {
+              const int x = c * S::B_COLS + q * 64, y = term * p.row_cap + w.row0;
+              if (full)
+                tma_load_2d(dst, &x_map_full, x, y, &ctl->b_full[st], pol);
+              else
+                for (int i = 0; i < boxes; ++i)
+                  tma_load_2d(dst + i * WM_BOX_TOK * 128, &x_map, x, y + i * WM_BOX_TOK, &ctl->b_full[st], pol);
             }
-            mbar_arrive_expect_tx(&ctl->b_full[st], full ? S::B_BYTES : boxes * WM_BOX_TOK * 128);
-            if (full)
-              tma_load_2d(ring_b + st * S::B_BYTES, &x_map_full, b * 64, term * p.row_cap + w.row0, &ctl->b_full[st], pol);
-            else
-            for (int i = 0; i < boxes; ++i)
-              tma_load_2d(ring_b + st * S::B_BYTES + i * WM_BOX_TOK * 128, &x_map, b * 64,
-                          term * p.row_cap + w.row0 + i * WM_BOX_TOK, &ctl->b_full[st], pol);
-          }
+        }
       }
       if (*abort_flag)
-        for (uint32_t i = 1; i <= WM_B_STAGES && i <= it; ++i)
-          mbar_wait_drain(&ctl->b_full[(it - i) % WM_B_STAGES], ((it - i) / WM_B_STAGES) & 1u);
+        for (uint32_t i = 1; i <= S::B_STAGES && i <= it; ++i)
+          mbar_wait_drain(&ctl->b_full[(it - i) % S::B_STAGES], ((it - i) / S::B_STAGES) & 1u);
     } else if (warp == 1 && elect_one()) {
       // ---------------- mma ----------------
       const uint64_t b_desc0 = sdesc_k_sw128(smem_u32(ring_b));
@@ -316,67 +330,46 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         const int n = (w.tokens + 15) & ~15;
         constexpr uint32_t fmt = std::is_same_v<W, __half> ? 0u : (1u << 7) | (1u << 10);
         const uint32_t idesc = (1u << 4) | fmt | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
-        const int blocks = min((p.K + 63) / 64, 2 * s1) - 2 * s0;
-        // One block of 64 columns; LAST: the last of its step. An accumulator covers one block (group 64), the two
-        // of a step (128) or half a block (32).
-        auto block = [&](int b, uint32_t a, bool first, bool last) {
-#pragma unroll
-          for (int term = 0; term < TERMS; ++term) {
-            const uint32_t e = b_it + term;
-            ok = ok && mbar_wait_spin(&ctl->b_full[e % WM_B_STAGES], (e / WM_B_STAGES) & 1u, abort_flag, ST_TIMEOUT_MMA);
-          }
-          auto open = [&]() {
-            const uint32_t q = d_it % S::BUFS;
-            ok = ok && mbar_wait_spin(&ctl->d_empty[q], ((d_it / S::BUFS) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA);
-          };
-          auto close = [&]() {
-            tc_commit(&ctl->d_full[d_it % S::BUFS]);
-            ++d_it;
-          };
-          if (p.w.group >= 64) {
-            const bool opens = first || p.w.group == 64;
-            if (opens) open();
-            if (!ok) return;
-            tc_fence_after();
-            const uint32_t d = tmem + (d_it % S::BUFS) * NT;
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-              const uint64_t bd = b_desc0 + ((b_it + term) % WM_B_STAGES) * (S::B_BYTES >> 4);
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, opens && term == 0 && kk == 0 ? 0u : 1u);
-            }
-            if (last || p.w.group == 64) close();
-          } else {
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              if ((2 * s0 + b) * 64 + part * 32 < p.K) {
-                open();
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t d = tmem + (d_it % S::BUFS) * NT;
-#pragma unroll
-                for (int term = 0; term < TERMS; ++term) {
-                  const uint64_t bd = b_desc0 + ((b_it + term) % WM_B_STAGES) * (S::B_BYTES >> 4);
-#pragma unroll
-                  for (int kk = 2 * part; kk < 2 * part + 2; ++kk)
-                    tc_mma_ts(d, a + kk * 8, bd + kk * 2, idesc, term == 0 && kk == 2 * part ? 0u : 1u);
-                }
-                close();
-              }
-            }
-          }
-#pragma unroll
-          for (int term = 0; term < TERMS; ++term, ++b_it)
-            tc_commit(&ctl->b_empty[b_it % WM_B_STAGES]);
-        };
-        for (int b = 0; b < blocks && ok; b += 2, ++a_it) {
+        for (int s = s0; s < s1 && ok; ++s, ++a_it) {
           const uint32_t slot = a_it % WM_A_SLOTS;
           ok = mbar_wait_spin(&ctl->a_full[slot], (a_it / WM_A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA);
-          if (!ok) break;
-          const uint32_t a = tmem + WM_A_COL + slot * 64;
-          block(b, a, true, b + 1 == blocks);
-          if (ok && b + 1 < blocks) block(b + 1, a + 32, false, true);
+          const uint32_t a = tmem + WM_A_COL + slot * 128;
+          uint64_t bd = b_desc0;
+          uint32_t d = 0;
+#pragma unroll
+          for (int c = 0; c < WM_STEP / 64 && ok; ++c) {               // 64 columns at a time
+            if (c % (S::B_COLS / 64) == 0) {
+              ok = mbar_wait_spin(&ctl->b_full[b_it % S::B_STAGES], (b_it / S::B_STAGES) & 1u, abort_flag, ST_TIMEOUT_MMA);
+              bd = b_desc0 + (b_it % S::B_STAGES) * (S::B_BYTES >> 4);
+            }
+            constexpr int PARTS = G == 32 ? 2 : 1;                     // groups that share these 64 columns
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+              const int k = c * 64 + part * 32;                        // column of the step
+              if (k % (G * GPB) == 0) {                                // a batch of accumulators starts
+                ok = ok && mbar_wait_spin(&ctl->d_empty[d_it & 1], ((d_it >> 1) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA);
+                d = tmem + (d_it & 1) * WM_D_COLS;
+              }
+              if (k % (G * GPB) == 0 || c % (S::B_COLS / 64) == 0) tc_fence_after();
+              if (ok) {
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                  for (int kk = 0; kk < 4 / PARTS; ++kk) {
+                    const int k16 = part * (4 / PARTS) + kk;           // 16 columns of the 64
+                    tc_mma_ts(d + ((k / G) % GPB) * NT, a + c * 32 + k16 * 8,
+                              bd + ((term * (S::B_COLS / 64) + c % (S::B_COLS / 64)) * NT * 128 >> 4) + k16 * 2, idesc,
+                              k % G == 0 && term == 0 && kk == 0 ? 0u : 1u);
+                  }
+                if ((k + 64 / PARTS) % (G * GPB) == 0) tc_commit(&ctl->d_full[d_it & 1]);
+              }
+              if ((k + 64 / PARTS) % (G * GPB) == 0) ++d_it;
+            }
+            if ((c + 1) % (S::B_COLS / 64) == 0) {
+              if (ok) tc_commit(&ctl->b_empty[b_it % S::B_STAGES]);
+              ++b_it;
+            }
+          }
           if (ok) tc_commit(&ctl->a_empty[slot]);
         }
       }
@@ -385,15 +378,17 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       mbar_wait_drain(&ctl->mma_done, 0);
     }
   } else if (warp < 12) {
-    // ---------------- codes to numbers ----------------
+    // ---------------- codes to numbers: the warpgroups take turns with the steps ----------------
     if constexpr (NT == 128) regs_dec<WM_REGS_CONV>();
-    const int wg = (warp - 4) >> 2, q4 = warp & 3;
+    const uint32_t wg = (warp - 4) >> 2;
+    const int q4 = warp & 3;
     // Row of the shared tile behind this lane of tensor memory; `up` puts X1's 16 rows and X2's side by side.
     const int srow = MODE == WS_UP ? (lane >> 4) * 64 + q4 * 16 + (lane & 15) : q4 * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
-    uint32_t c_it = 0, a_base = 0;
-    bool stop = false;
-    for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
+    const uint32_t a_dst = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + WM_A_COL + wg * 128;
+    const uint8_t* row = ring_c + srow * 128;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
       int s0, s1;
       range(w, s0, s1);
@@ -404,50 +399,40 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
             : static_cast<long long>(w.expert) * p.N + min(w.rt * 128 + srow, p.N - 1);
         zrow = p.w.zero + r * groups;
       }
-      for (int s = s0; s < s1; s += 2, ++c_it) {
-        const int mine = s + wg;
-        const bool valid = mine < s1;
-        uint32_t off[4];
+      for (int s = s0; s < s1 && ok; ++s, ++it) {
+        if ((it & 1u) != wg) continue;
+        uint32_t off[GPS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          int z = 8;
-          if (zrow != nullptr && valid) z = __ldg(zrow + min((mine * 128 + i * 32) / p.w.group, groups - 1)) & 15;
-          off[i] = w4_offset<W>(z);
-        }
-        const int st = c_it % S::CODE_STAGES;
-        const uint32_t ph = (c_it / S::CODE_STAGES) & 1u;
-        if (!mbar_wait_warp(&ctl->c_full[st], ph, abort_flag, ST_TIMEOUT_EPILOGUE)) { stop = true; break; }
-        mbar_observe(&ctl->c_full[st], ph);
-        uint4 v[4];
-        const uint8_t* row = ring_c + st * WM_CODE_BYTES + srow * 128;
+        for (int i = 0; i < GPS; ++i) off[i] = w4_offset<W>(zrow ? __ldg(zrow + min(s * GPS + i, groups - 1)) & 15 : 8);
+        const uint32_t st = it % S::CODE_STAGES;
+        if (!wait_warp(&ctl->c_full[st], (it / S::CODE_STAGES) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { ok = false; break; }
+        uint4 v[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = *reinterpret_cast<const uint4*>(row + (((wg * 4 + c) ^ (srow & 7)) << 4));
+        for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const uint4*>(row + st * WM_CODE_BYTES + ((c ^ (srow & 7)) << 4));
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->c_empty[st]);
-        if (!valid) continue;
-        const uint32_t a_it = a_base + static_cast<uint32_t>(mine - s0), slot = a_it % WM_A_SLOTS;
-        if (!mbar_wait_warp(&ctl->a_empty[slot], ((a_it / WM_A_SLOTS) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { stop = true; break; }
+        if (!wait_warp(&ctl->a_empty[wg], ((it >> 1) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int hf = 0; hf < 4; ++hf) {                               // 64 columns: 32 columns of tensor memory
           uint32_t r[32];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const uint32_t o = off[hf * 2 + c];
-            const uint32_t word[4] = {v[hf * 2 + c].x, v[hf * 2 + c].y, v[hf * 2 + c].z, v[hf * 2 + c].w};
+            const uint32_t o = off[(hf * 64 + c * 32) / G];
+            const uint4 x = v[hf * 2 + c];
+            const uint32_t word[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
               for (int j = 0; j < 4; ++j) r[c * 16 + i * 4 + j] = w4_pair<W>(word[i], j, o);
           }
-          tmem_st32(tmem + lanes + WM_A_COL + slot * 64 + hf * 32, r);
+          tmem_st32(a_dst + hf * 32, r);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->a_full[slot]);
+        if (lane == 0) mbar_arrive(&ctl->a_full[wg]);
       }
-      a_base += static_cast<uint32_t>(s1 - s0);
     }
   } else {
     // ---------------- scale and store ----------------
@@ -460,29 +445,37 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
       int s0, s1;
       range(w, s0, s1);
-      const int g0 = s0 * 128 / p.w.group, g1 = min(groups, s1 * 128 / p.w.group);
       const int col = MODE == WS_UP ? w.rt * 64 + q4 * 16 + (lane & 15) : w.rt * 128 + q4 * 32 + lane;
       const long long mrow = MODE == WS_UP ? static_cast<long long>(w.expert) * 2 * p.N + (lane >> 4) * static_cast<long long>(p.N) + min(col, p.N - 1)
                                            : static_cast<long long>(w.expert) * p.N + min(col, p.N - 1);
       const T* srow = static_cast<const T*>(p.w.scale) + mrow * groups;
+      // Scales of the next batch, in flight while this one is waited for; 0 past the last group.
+      auto scales = [&](int g, float (&f)[GPB]) {
+#pragma unroll
+        for (int i = 0; i < GPB; ++i) f[i] = g + i < groups ? to_f32(srow[g + i]) : 0.0f;
+      };
       float total[NT];
 #pragma unroll
       for (int i = 0; i < NT; ++i) total[i] = 0.0f;
-      float next = to_f32(srow[g0]);
-      for (int g = g0; g < g1; ++g, ++d_it) {
-        const float f = next;
-        if (g + 1 < g1) next = to_f32(srow[g + 1]);
-        const uint32_t q = d_it % S::BUFS, ph = (d_it / S::BUFS) & 1u;
-        if (!mbar_wait_warp(&ctl->d_full[q], ph, abort_flag, ST_TIMEOUT_EPILOGUE, true)) { stop = true; break; }
-        mbar_observe(&ctl->d_full[q], ph);
+      float next[GPB];
+      scales(s0 * GPS, next);
+      for (int g = s0 * GPS; g < s1 * GPS; g += GPB, ++d_it) {
+        float f[GPB];
+#pragma unroll
+        for (int i = 0; i < GPB; ++i) f[i] = next[i];
+        scales(g + GPB, next);
+        const uint32_t q = d_it & 1;
+        if (!wait_warp(&ctl->d_full[q], (d_it >> 1) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { stop = true; break; }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < NT / 32; ++c)
-          if (c * 32 < w.tokens) {
-            float v[32];
-            tmem_ld32(tmem + lanes + q * NT + c * 32, v);
-            fma32_scaled(total + c * 32, v, f);
-          }
+        for (int i = 0; i < GPB; ++i)
+#pragma unroll
+          for (int c = 0; c < NT / 32; ++c)
+            if (c * 32 < w.tokens) {
+              float v[32];
+              tmem_ld32(tmem + lanes + q * WM_D_COLS + i * NT + c * 32, v);
+              fma32_scaled(total + c * 32, v, f[i]);
+            }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->d_empty[q]);
