@@ -700,7 +700,7 @@ LinearW4Ws make_linear_w4_ws(int M, int N, int K) {
     off = ws_align(off + n);
     return o;
   };
-  w.x = take(static_cast<size_t>(M) * round_up(K, 8) * 2);
+  w.x = take(static_cast<size_t>(M) * round_up(K, 64) * 2);
   const int splits = wm_splits(M, N, K);
   w.parts = take(splits > 1 ? sizeof(float) * splits * static_cast<size_t>(M) * N : 0);
   // The copy of the codes is only used where their own rows do not allow TMA; a base that is not 16-byte aligned
@@ -728,8 +728,8 @@ ExpertsW4Ws make_experts_w4_ws(int T, int k, int E, int H, int I) {
   } else {
     w.counts = take(sizeof(int) * E);
     w.slot = take(sizeof(int) * routes);
-    w.x = take(routes * round_up(H, 8) * 2);
-    w.h = take(routes * round_up(I, 8) * 4);
+    w.x = take(routes * round_up(H, 64) * 2);
+    w.h = take(routes * round_up(I, 64) * 4);
     w.y = take(routes * H * 4);
     // Copies of codes whose rows do not allow TMA (odd widths).
     w.c13 = take(w4_bytes(H) % 16 ? static_cast<size_t>(E) * 2 * I * round_up(w4_bytes(H), 16) : 0);
@@ -739,16 +739,20 @@ ExpertsW4Ws make_experts_w4_ws(int T, int k, int E, int H, int I) {
   return w;
 }
 
-// Tensor map of a 2-D array of rows `pitch` bytes apart, 128-byte swizzle, boxes of 128 bytes x `box_rows`.
-int w4_map(CUtensorMapDataType type, const void* base, long long width, long long rows, long long pitch, int box_width, int box_rows,
+// 4-D tensor map with the 128-byte swizzle; strides in bytes of dimensions 1 to 3.
+int w4_map(CUtensorMapDataType type, const void* base, const long long (&dims)[4], const long long (&strides)[3], const int (&box)[4],
            CUtensorMap* map) {
   PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_width), static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t elem[2] = {1, 1};
-  const CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4];
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    b[i] = static_cast<cuuint32_t>(box[i]);
+    if (i < 3) s[i] = static_cast<cuuint64_t>(strides[i]);
+  }
+  const CUresult r = encode(map, type, 4, const_cast<void*>(base), d, s, b, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(r));
   return MOE_OK;
@@ -775,25 +779,32 @@ int wm_prepare(int smem, bool split_regs) {
 }
 
 template <typename T, int MODE, int NT, int G>
-int launch_w4_mma_g(DeviceInfo* d, const CUtensorMap& cm, const CUtensorMap& xm, const CUtensorMap& xf, const WmArgs& a, long long units,
-                    cudaStream_t st) {
+int launch_w4_mma_g(DeviceInfo* d, const WmMaps& maps, const WmArgs& a, long long units, cudaStream_t st) {
   constexpr int smem = WM_SMEM<NT, MODE == WS_DOWN ? 2 : 1>;
   if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT, G>>(smem, NT == 128)) return rc;
   const int grid = units < d->num_sms ? static_cast<int>(units) : d->num_sms;
-  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT, G>, grid < 1 ? 1 : grid, WM_THREADS, smem, st, cm, xm, xf, a),
+  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT, G>, grid < 1 ? 1 : grid, WM_THREADS, smem, st, maps, a),
                     "w4_mma launch");
 }
 
 // x_rows: rows of the token buffer; tile: tokens per tile.
 template <typename T, int MODE, int NT>
 int launch_w4_mma_nt(DeviceInfo* d, const WmArgs& a, const void* x, long long x_rows, cudaStream_t st) {
-  const int pitch = round_up(w4_bytes(a.K), 16), width = round_up(a.K, 8);
-  const long long rows = static_cast<long long>(a.E) * (MODE == WS_UP ? 2 : 1) * a.N;
-  CUtensorMap cm, xm, xf;
-  if (int rc = w4_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w.codes, pitch, rows, pitch, 128, 64, &cm)) return rc;
+  constexpr int TERMS = MODE == WS_DOWN ? 2 : 1, HALVES = MODE == WS_UP ? 2 : 1;
+  WmMaps maps;
+  {
+    const long long pitch = round_up(w4_bytes(a.K), 16);
+    const long long dims[4] = {pitch, a.N, HALVES, a.E}, strides[3] = {pitch, pitch * a.N, pitch * a.N * HALVES};
+    const int box[4] = {WM_STEP / 2, 128 / HALVES, HALVES, 1};
+    if (int rc = w4_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w.codes, dims, strides, box, &maps.codes)) return rc;
+  }
   const CUtensorMapDataType t = MODE != WS_DOWN && std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, WM_BOX_TOK, &xm)) return rc;
-  if (int rc = w4_map(t, x, width, x_rows, width * 2ll, 64, NT, &xf)) return rc;
+  for (int i = 0; i < 4 && (16 << i) <= NT; ++i) {
+    const long long pitch = round_up(a.K, 64) * 2ll, rows = x_rows / TERMS;
+    const long long dims[4] = {64, rows, TERMS, pitch / 128}, strides[3] = {pitch, pitch * rows, 128};
+    const int box[4] = {64, 16 << i, TERMS, WmShape<NT, TERMS>::B_COLS / 64};
+    if (int rc = w4_map(t, x, dims, strides, box, &maps.x[i])) return rc;
+  }
   const int per = MODE == WS_UP ? 64 : 128;
   // Most units that there can be: every expert's tokens in tiles, or one token in each.
   const long long row_tiles = (static_cast<long long>(a.N) + per - 1) / per;
@@ -801,9 +812,9 @@ int launch_w4_mma_nt(DeviceInfo* d, const WmArgs& a, const void* x, long long x_
   const long long tiles = MODE == WS_LINEAR ? (tokens + NT - 1) / NT : (tokens < a.E ? tokens : a.E) + tokens / NT;
   const long long units = tiles * row_tiles * a.splits;
   switch (a.w.group) {
-    case 32: return launch_w4_mma_g<T, MODE, NT, 32>(d, cm, xm, xf, a, units, st);
-    case 64: return launch_w4_mma_g<T, MODE, NT, 64>(d, cm, xm, xf, a, units, st);
-    default: return launch_w4_mma_g<T, MODE, NT, 128>(d, cm, xm, xf, a, units, st);
+    case 32: return launch_w4_mma_g<T, MODE, NT, 32>(d, maps, a, units, st);
+    case 64: return launch_w4_mma_g<T, MODE, NT, 64>(d, maps, a, units, st);
+    default: return launch_w4_mma_g<T, MODE, NT, 128>(d, maps, a, units, st);
   }
 }
 
@@ -844,7 +855,7 @@ int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Mat
   WmArgs a{};
   a.w = w;
   if (int rc = w4_tma_codes(d, w.codes, N, K, W + ws.codes, &a.w.codes, st)) return rc;
-  pair_rows_kernel<T><<<grid_for(static_cast<size_t>(M) * (round_up(K, 8) / 8), 256, d->num_sms * 8), 256, 0, st>>>(
+  pair_rows_kernel<T><<<grid_for(static_cast<size_t>(M) * (round_up(K, 64) / 8), 256, d->num_sms * 8), 256, 0, st>>>(
       static_cast<const T*>(x), x_stride, M, K, reinterpret_cast<T*>(W + ws.x));
   a.E = 1;
   a.N = N;
@@ -915,7 +926,7 @@ int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W
   up.sps = (up.K + WM_STEP - 1) / WM_STEP;
   down.sps = (down.K + WM_STEP - 1) / WM_STEP;
   up.h = h;
-  up.h_pitch = round_up(p.I, 8);
+  up.h_pitch = round_up(p.I, 64);
   down.y = y;
   const int tile = wm_tile((routes + p.E - 1) / p.E);
   if (int rc = launch_w4_mma<T, WS_UP>(d, up, xg, routes, tile, st)) return rc;

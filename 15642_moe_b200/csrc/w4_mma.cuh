@@ -25,17 +25,17 @@ namespace moe {
 constexpr int WM_THREADS = 512;
 constexpr int WM_STEP = 256;                    // columns per step
 constexpr int WM_CODE_BYTES = 128 * WM_STEP / 2;
-constexpr int WM_A_SLOTS = 2;                   // steps in tensor memory (128 of its columns each), one per warpgroup
-constexpr int WM_A_COL = 256;                   // accumulators in [0, 256), weights in [256, 512)
-constexpr int WM_D_COLS = 128;                  // columns of one batch of accumulators, two batches
-constexpr int WM_BOX_TOK = 16;                  // token rows per small TMA box
 constexpr int WM_REGS_CTRL = 48, WM_REGS_CONV = 104, WM_REGS_EPI = 232;   // register split for NT = 128
 constexpr int WM_LAUNCH_REGS_MIN = (WM_REGS_CTRL + 2 * WM_REGS_CONV + WM_REGS_EPI + 3) / 4;
 
 // Shared memory: a ring of steps of codes, a ring of token rows. An entry of the second holds B_COLS columns of every
 // term (up to 64 KB), so that a step of few tokens is one entry.
+// Tensor memory: two batches of accumulators, then the weights of as many steps (128 columns each) as fit.
 template <int NT, int TERMS>
 struct WmShape {
+  static constexpr int D_COLS = NT * TERMS >= 64 ? 128 : 64;
+  static constexpr int A_COL = 2 * D_COLS;
+  static constexpr int A_SLOTS = (512 - A_COL) / 128;
   static constexpr int B_COLS = NT * TERMS >= 128 ? 128 : 256;
   static constexpr int B_BYTES = NT * TERMS * B_COLS * 2;
   static constexpr int B_STAGES = 4;
@@ -47,7 +47,7 @@ struct WmShape {
 struct WmCtrl {
   uint64_t c_full[8], c_empty[8];
   uint64_t b_full[4], b_empty[4];
-  uint64_t a_full[WM_A_SLOTS], a_empty[WM_A_SLOTS];
+  uint64_t a_full[3], a_empty[3];
   uint64_t d_full[2], d_empty[2];
   uint64_t mma_done;
   uint32_t tmem_base;
@@ -58,6 +58,14 @@ struct WmCtrl {
 
 template <int NT, int TERMS>
 constexpr int WM_SMEM = WmShape<NT, TERMS>::RING + static_cast<int>(sizeof(WmCtrl)) + 1024;
+
+// Tensor maps. codes: 4-D (bytes of a row, rows, X1 / X2, experts), one box per step. x: 4-D (64 columns, rows, terms,
+// blocks of 64 columns), one map for each box height of 16, 32, 64, 128 rows; a box is a ring entry as the mma reads it.
+// One copy instruction per entry: a producer's thread needs some hundred cycles for each.
+struct WmMaps {
+  CUtensorMap codes;
+  CUtensorMap x[4];
+};
 
 struct WmArgs {
   W4Matrix w;
@@ -98,6 +106,15 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
       : "memory");
 }
 
+// 4-D tiled TMA load (no multicast) with an L2 policy.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
 // One lane of a converged warp. The compiler then knows that a single thread runs what follows and keeps the operands of
 // mma and copy instructions in uniform registers: an mma with 16 tokens issues every 9 cycles, behind `lane == 0` every 46.
 __device__ __forceinline__ bool elect_one() {
@@ -110,10 +127,10 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// Bounded wait by polling, all lanes of a converged warp; they agree on giving up.
+// Bounded wait of a converged warp, every lane for itself (each needs its own acquire); they agree on giving up. The
+// hardware suspends the lanes meanwhile: polling warps take issue slots and shared-memory cycles from the others.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int who) {
-  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
-  return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, abort_flag, who));
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, who));
 }
 
 // Tiles of up to NT tokens: an expert's rows in equal parts.
@@ -162,6 +179,9 @@ __device__ __forceinline__ void wm_build_map(int* tile_off, int* row_off, const 
   }
 }
 
+// Operand columns of a tile's tokens, 16 << wm_box(tokens): the height of the box that brings them.
+__device__ __forceinline__ int wm_box(int tokens) { return (tokens > 16) + (tokens > 32) + (tokens > 64); }
+
 struct WmUnit {
   int expert, row0, tokens;    // first row and count of the tile's tokens
   int rt, split;               // 128-row tile of the weights; part of the columns
@@ -190,14 +210,13 @@ __device__ __forceinline__ WmUnit wm_unit(const WmCtrl* ctl, const WmArgs& p, in
 
 template <typename T, int MODE, int NT, int G>
 __global__ void __launch_bounds__(WM_THREADS, 1)
-    w4_mma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map,
-                  const __grid_constant__ CUtensorMap x_map_full, const __grid_constant__ WmArgs p) {
+    w4_mma_kernel(const __grid_constant__ WmMaps maps, const __grid_constant__ WmArgs p) {
   using W = typename std::conditional<MODE == WS_DOWN, __nv_bfloat16, T>::type;   // the operands' type
   constexpr int TERMS = MODE == WS_DOWN ? 2 : 1;
   using S = WmShape<NT, TERMS>;
   constexpr int GPS = WM_STEP / G;                                      // groups per step
-  constexpr int GPB = WM_D_COLS / NT < GPS ? WM_D_COLS / NT : GPS;      // groups per batch of accumulators
-  constexpr int BATCHES = GPS / GPB;                                    // batches per step
+  constexpr int NC = NT * TERMS;                                        // columns of one accumulator
+  constexpr int GPB = S::D_COLS / NC < GPS ? S::D_COLS / NC : GPS;      // groups per batch of accumulators
   constexpr int ENTRIES = WM_STEP / S::B_COLS;                          // entries of token rows per step
   extern __shared__ uint8_t wm_raw[];
   uint8_t* smem = align_1024(wm_raw);
@@ -215,7 +234,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       mbar_init(&ctl->b_full[i], 1);
       mbar_init(&ctl->b_empty[i], 1);
     }
-    for (int i = 0; i < WM_A_SLOTS; ++i) {
+    for (int i = 0; i < S::A_SLOTS; ++i) {
       mbar_init(&ctl->a_full[i], 4);
       mbar_init(&ctl->a_empty[i], 1);
     }
@@ -270,15 +289,12 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
         int s0, s1;
         range(w, s0, s1);
-        const int y0 = MODE == WS_UP ? w.expert * 2 * p.N + w.rt * 64 : w.expert * p.N + w.rt * 128;
-        const int y1 = MODE == WS_UP ? y0 + p.N : y0 + 64;
+        const int y = w.rt * per_tile;
         for (int s = s0; s < s1; ++s, ++it) {
           const int st = it % S::CODE_STAGES;
           if (!mbar_wait(&ctl->c_empty[st], ((it / S::CODE_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) break;
           mbar_arrive_expect_tx(&ctl->c_full[st], WM_CODE_BYTES);
-          uint8_t* dst = ring_c + st * WM_CODE_BYTES;
-          tma_load_2d(dst, &code_map, s * (WM_STEP / 2), y0, &ctl->c_full[st], pol);
-          tma_load_2d(dst + WM_CODE_BYTES / 2, &code_map, s * (WM_STEP / 2), y1, &ctl->c_full[st], pol);
+          tma_load_4d(ring_c + st * WM_CODE_BYTES, &maps.codes, s * (WM_STEP / 2), y, 0, w.expert, &ctl->c_full[st], pol);
         }
       }
       if (*abort_flag)
@@ -293,26 +309,14 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
         int s0, s1;
         range(w, s0, s1);
-        // Few tokens: boxes of 16 rows; more than half a tile: one box (rows past the tile's are read for nothing).
-        const bool full = 2 * w.tokens > NT;
-        const int boxes = (w.tokens + WM_BOX_TOK - 1) / WM_BOX_TOK;
-        const uint32_t bytes = (full ? NT : boxes * WM_BOX_TOK) * S::B_COLS * 2 * TERMS;
+        const int box = wm_box(w.tokens);                    // rows past the tile's are read for nothing
+        const CUtensorMap* map = &maps.x[box];
+        const uint32_t bytes = (16u << box) * S::B_COLS * 2 * TERMS;
         for (int c = s0 * ENTRIES; c < s1 * ENTRIES; ++c, ++it) {
           const int st = it % S::B_STAGES;
           if (!mbar_wait(&ctl->b_empty[st], ((it / S::B_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) break;
           mbar_arrive_expect_tx(&ctl->b_full[st], bytes);
-          uint8_t* dst = ring_b + st * S::B_BYTES;
-#pragma unroll
-          for (int term = 0; term < TERMS; ++term)
-#pragma unroll
-            for (int q = 0; q < S::B_COLS / 64; ++q, dst += NT * 128) {
-              const int x = c * S::B_COLS + q * 64, y = term * p.row_cap + w.row0;
-              if (full)
-                tma_load_2d(dst, &x_map_full, x, y, &ctl->b_full[st], pol);
-              else
-                for (int i = 0; i < boxes; ++i)
-                  tma_load_2d(dst + i * WM_BOX_TOK * 128, &x_map, x, y + i * WM_BOX_TOK, &ctl->b_full[st], pol);
-            }
+          tma_load_4d(ring_b + st * S::B_BYTES, map, 0, w.row0, 0, c * (S::B_COLS / 64), &ctl->b_full[st], pol);
         }
       }
       if (*abort_flag)
@@ -320,59 +324,58 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
           mbar_wait_drain(&ctl->b_full[(it - i) % S::B_STAGES], ((it - i) / S::B_STAGES) & 1u);
     } else if (warp == 1 && elect_one()) {
       // ---------------- mma ----------------
+      constexpr int BC = S::B_COLS / 64, PARTS = G == 32 ? 2 : 1;      // 64-column pieces per entry, groups per piece
       const uint64_t b_desc0 = sdesc_k_sw128(smem_u32(ring_b));
       uint32_t b_it = 0, a_it = 0, d_it = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      // A wait that gives up leaves at once: a flag tested before each mma would double the cost of issuing it.
+      for (int u = blockIdx.x; u < units; u += gridDim.x) {
         const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
         int s0, s1;
         range(w, s0, s1);
-        const int n = (w.tokens + 15) & ~15;
+        const int n = TERMS * (16 << wm_box(w.tokens));
+        const uint64_t chunk = static_cast<uint64_t>(n * 128 >> 4);    // from one block of 64 columns to the next
         constexpr uint32_t fmt = std::is_same_v<W, __half> ? 0u : (1u << 7) | (1u << 10);
         const uint32_t idesc = (1u << 4) | fmt | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
-        for (int s = s0; s < s1 && ok; ++s, ++a_it) {
-          const uint32_t slot = a_it % WM_A_SLOTS;
-          ok = mbar_wait_spin(&ctl->a_full[slot], (a_it / WM_A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA);
-          const uint32_t a = tmem + WM_A_COL + slot * 128;
+        for (int s = s0; s < s1; ++s, ++a_it) {
+          const uint32_t slot = a_it % S::A_SLOTS;
+          if (!mbar_wait_spin(&ctl->a_full[slot], (a_it / S::A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA)) goto mma_end;
+          const uint32_t a = tmem + S::A_COL + slot * 128;
           uint64_t bd = b_desc0;
           uint32_t d = 0;
 #pragma unroll
-          for (int c = 0; c < WM_STEP / 64 && ok; ++c) {               // 64 columns at a time
-            if (c % (S::B_COLS / 64) == 0) {
-              ok = mbar_wait_spin(&ctl->b_full[b_it % S::B_STAGES], (b_it / S::B_STAGES) & 1u, abort_flag, ST_TIMEOUT_MMA);
+          for (int c = 0; c < WM_STEP / 64; ++c) {                     // 64 columns at a time
+            if (c % BC == 0) {
+              if (!mbar_wait_spin(&ctl->b_full[b_it % S::B_STAGES], (b_it / S::B_STAGES) & 1u, abort_flag, ST_TIMEOUT_MMA)) goto mma_end;
               bd = b_desc0 + (b_it % S::B_STAGES) * (S::B_BYTES >> 4);
             }
-            constexpr int PARTS = G == 32 ? 2 : 1;                     // groups that share these 64 columns
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) {
               const int k = c * 64 + part * 32;                        // column of the step
               if (k % (G * GPB) == 0) {                                // a batch of accumulators starts
-                ok = ok && mbar_wait_spin(&ctl->d_empty[d_it & 1], ((d_it >> 1) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA);
-                d = tmem + (d_it & 1) * WM_D_COLS;
+                if (!mbar_wait_spin(&ctl->d_empty[d_it & 1], ((d_it >> 1) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA)) goto mma_end;
+                d = tmem + (d_it & 1) * S::D_COLS;
               }
-              if (k % (G * GPB) == 0 || c % (S::B_COLS / 64) == 0) tc_fence_after();
-              if (ok) {
+              if (k % (G * GPB) == 0 || c % BC == 0) tc_fence_after();
 #pragma unroll
-                for (int term = 0; term < TERMS; ++term)
-#pragma unroll
-                  for (int kk = 0; kk < 4 / PARTS; ++kk) {
-                    const int k16 = part * (4 / PARTS) + kk;           // 16 columns of the 64
-                    tc_mma_ts(d + ((k / G) % GPB) * NT, a + c * 32 + k16 * 8,
-                              bd + ((term * (S::B_COLS / 64) + c % (S::B_COLS / 64)) * NT * 128 >> 4) + k16 * 2, idesc,
-                              k % G == 0 && term == 0 && kk == 0 ? 0u : 1u);
-                  }
-                if ((k + 64 / PARTS) % (G * GPB) == 0) tc_commit(&ctl->d_full[d_it & 1]);
+              for (int kk = 0; kk < 4 / PARTS; ++kk) {
+                const int k16 = part * (4 / PARTS) + kk;               // 16 columns of the 64
+                tc_mma_ts(d + ((k / G) % GPB) * NC, a + c * 32 + k16 * 8, bd + (c % BC) * chunk + k16 * 2, idesc,
+                          k % G == 0 && kk == 0 ? 0u : 1u);
               }
-              if ((k + 64 / PARTS) % (G * GPB) == 0) ++d_it;
+              if ((k + 64 / PARTS) % (G * GPB) == 0) {
+                tc_commit(&ctl->d_full[d_it & 1]);
+                ++d_it;
+              }
             }
-            if ((c + 1) % (S::B_COLS / 64) == 0) {
-              if (ok) tc_commit(&ctl->b_empty[b_it % S::B_STAGES]);
+            if ((c + 1) % BC == 0) {
+              tc_commit(&ctl->b_empty[b_it % S::B_STAGES]);
               ++b_it;
             }
           }
-          if (ok) tc_commit(&ctl->a_empty[slot]);
+          tc_commit(&ctl->a_empty[slot]);
         }
       }
+    mma_end:
       // Everything issued has finished before tensor and shared memory are given back.
       tc_commit(&ctl->mma_done);
       mbar_wait_drain(&ctl->mma_done, 0);
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
     const int q4 = warp & 3;
     // Row of the shared tile behind this lane of tensor memory; `up` puts X1's 16 rows and X2's side by side.
     const int srow = MODE == WS_UP ? (lane >> 4) * 64 + q4 * 16 + (lane & 15) : q4 * 32 + lane;
-    const uint32_t a_dst = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + WM_A_COL + wg * 128;
+    const uint32_t a_dst0 = tmem + (static_cast<uint32_t>(q4 * 32) << 16) + S::A_COL;
     const uint8_t* row = ring_c + srow * 128;
     uint32_t it = 0;
     bool ok = true;
@@ -401,25 +404,25 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       }
       for (int s = s0; s < s1 && ok; ++s, ++it) {
         if ((it & 1u) != wg) continue;
+        const uint32_t st = it % S::CODE_STAGES, slot = it % S::A_SLOTS;
         uint32_t off[GPS];
 #pragma unroll
         for (int i = 0; i < GPS; ++i) off[i] = w4_offset<W>(zrow ? __ldg(zrow + min(s * GPS + i, groups - 1)) & 15 : 8);
-        const uint32_t st = it % S::CODE_STAGES;
-        if (!wait_warp(&ctl->c_full[st], (it / S::CODE_STAGES) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { ok = false; break; }
-        uint4 v[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const uint4*>(row + st * WM_CODE_BYTES + ((c ^ (srow & 7)) << 4));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->c_empty[st]);
-        if (!wait_warp(&ctl->a_empty[wg], ((it >> 1) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { ok = false; break; }
+        if (!wait_warp(&ctl->c_full[st], (it / S::CODE_STAGES) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE) ||
+            !wait_warp(&ctl->a_empty[slot], ((it / S::A_SLOTS) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
+        const uint8_t* src = row + st * WM_CODE_BYTES;
+        const uint32_t a_dst = a_dst0 + slot * 128;
 #pragma unroll
         for (int hf = 0; hf < 4; ++hf) {                               // 64 columns: 32 columns of tensor memory
           uint32_t r[32];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + (((hf * 2 + c) ^ (srow & 7)) << 4));
             const uint32_t o = off[(hf * 64 + c * 32) / G];
-            const uint4 x = v[hf * 2 + c];
             const uint32_t word[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -428,10 +431,12 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
           }
           tmem_st32(a_dst + hf * 32, r);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->c_empty[st]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->a_full[wg]);
+        if (lane == 0) mbar_arrive(&ctl->a_full[slot]);
       }
     }
   } else {
@@ -472,9 +477,12 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
 #pragma unroll
           for (int c = 0; c < NT / 32; ++c)
             if (c * 32 < w.tokens) {
-              float v[32];
-              tmem_ld32(tmem + lanes + q * WM_D_COLS + i * NT + c * 32, v);
-              fma32_scaled(total + c * 32, v, f[i]);
+#pragma unroll
+              for (int term = 0; term < TERMS; ++term) {
+                float v[32];
+                tmem_ld32(tmem + lanes + q * S::D_COLS + i * NC + term * (16 << wm_box(w.tokens)) + c * 32, v);
+                fma32_scaled(total + c * 32, v, f[i]);
+              }
             }
         tc_fence_before();
         __syncwarp();
@@ -501,7 +509,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
         }
       } else {
         // Lanes 0-15 hold X1, lanes 16-31 X2 of the same columns: even tokens end in the first, odd in the second.
-        // hi + lo bf16 carry 16 bits of h; the columns go in pair order, zeros up to the next 8.
+        // hi + lo bf16 carry 16 bits of h; the columns go in pair order, zeros up to the next 64.
         const int pos = pair_pos(col), mine = lane >> 4;
 #pragma unroll
         for (int i = 0; i < NT; i += 2)
@@ -510,7 +518,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
             const float got = __shfl_xor_sync(0xffffffffu, give, 16);
             const float u1 = mine ? got : total[i], u2 = mine ? total[i + 1] : got;
             const float hv = col < p.N ? u1 * (u2 / (1.0f + expf(-u2))) : 0.0f;
-            if (i + mine < w.tokens && pos < p.h_pitch) {
+            if (i + mine < w.tokens) {
               const __nv_bfloat16 hi = __float2bfloat16_rn(hv);
               const float rest = hv - __bfloat162float(hi);
               const long long at = static_cast<long long>(w.row0 + i + mine) * p.h_pitch + pos;
@@ -546,11 +554,11 @@ __device__ __forceinline__ uint4 ld_pairs(const T* row, int k, int K) {
   return *reinterpret_cast<const uint4*>(o);
 }
 
-// Rows of x in pair order, columns padded with zeros to a multiple of 8.
+// Rows of x in pair order, columns padded with zeros to a multiple of 64.
 template <typename T>
 __global__ void __launch_bounds__(256) pair_rows_kernel(const T* x, long long x_stride, int M, int K, T* out) {
   allow_dependent_launch();
-  const int per = (K + 7) / 8;
+  const int per = (K + 63) / 64 * 8;
   const long long n = static_cast<long long>(M) * per;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const long long m = i / per;
@@ -600,7 +608,7 @@ __global__ void __launch_bounds__(256) experts_gather_kernel(const T* x, long lo
   allow_dependent_launch();
   if (threadIdx.x < 32) wm_build_map(tile_off, row_off, counts, E, n, 128);
   __syncthreads();
-  const int per = (H + 7) / 8, lane = threadIdx.x & 31;
+  const int per = (H + 63) / 64 * 8, lane = threadIdx.x & 31;
   for (int r = (blockIdx.x * 256 + threadIdx.x) >> 5; r < n; r += gridDim.x * 8) {
     const int s = slot[r];
     if (s < 0) continue;
