@@ -781,9 +781,9 @@ int wm_prepare(int smem, bool split_regs) {
 template <typename T, int MODE, int NT, int G>
 int launch_w4_mma_g(DeviceInfo* d, const WmMaps& maps, const WmArgs& a, long long units, cudaStream_t st) {
   constexpr int smem = WM_SMEM<NT, MODE == WS_DOWN ? 2 : 1>;
-  if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT, G>>(smem, NT == 128)) return rc;
+  if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT, G>>(smem, NT > 32)) return rc;
   const int grid = units < d->num_sms ? static_cast<int>(units) : d->num_sms;
-  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT, G>, grid < 1 ? 1 : grid, WM_THREADS, smem, st, maps, a),
+  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT, G>, grid < 1 ? 1 : grid, WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS, smem, st, maps, a),
                     "w4_mma launch");
 }
 

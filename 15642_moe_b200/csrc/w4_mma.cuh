@@ -12,8 +12,8 @@
  * A word's codes come out as the pairs (0,4), (1,5), (2,6), (3,7) with two instructions each; the tokens' rows are
  * kept in that order of columns (within each 8), which costs their copy nothing.
  *
- * Roles (16 warps): warp 0 loads codes, warp 1 issues the mma, warp 2 loads token rows, warps 4-11 convert (two
- * warpgroups take turns with steps of 128 columns), warps 12-15 scale and store. Persistent: one block per SM walks
+ * Roles: warp 0 loads codes, warp 1 issues the mma, warp 2 loads token rows; two warpgroups convert, taking turns with
+ * steps of 256 columns; one or two scale and store. Persistent: one block per SM walks
  * the units (token tile, 128 weight rows[, part of the columns]).
  */
 #pragma once
@@ -22,20 +22,24 @@
 
 namespace moe {
 
-constexpr int WM_THREADS = 512;
 constexpr int WM_STEP = 256;                    // columns per step
 constexpr int WM_CODE_BYTES = 128 * WM_STEP / 2;
-constexpr int WM_REGS_CTRL = 48, WM_REGS_CONV = 104, WM_REGS_EPI = 232;   // register split for NT = 128
-constexpr int WM_LAUNCH_REGS_MIN = (WM_REGS_CTRL + 2 * WM_REGS_CONV + WM_REGS_EPI + 3) / 4;
+// Register split of the blocks of 640 threads: warpgroup 0, the two that convert, the two that scale.
+constexpr int WM_REGS_CTRL = 40, WM_REGS_CONV = 88, WM_REGS_EPI = 128;
+constexpr int WM_LAUNCH_REGS_MIN = (WM_REGS_CTRL + 2 * WM_REGS_CONV + 2 * WM_REGS_EPI + 4) / 5;
 
 // Shared memory: a ring of steps of codes, a ring of token rows. An entry of the second holds B_COLS columns of every
 // term (up to 64 KB), so that a step of few tokens is one entry.
 // Tensor memory: two batches of accumulators, then the weights of as many steps (128 columns each) as fit.
 template <int NT, int TERMS>
 struct WmShape {
-  static constexpr int D_COLS = NT * TERMS >= 64 ? 128 : 64;
+  static constexpr int D_COLS = NT * TERMS >= 128 ? 128 : 64;
   static constexpr int A_COL = 2 * D_COLS;
   static constexpr int A_SLOTS = (512 - A_COL) / 128;
+  // Warpgroups that scale, each TOK tokens of the tile: above 32 tokens one would be the slowest of the roles.
+  static constexpr int EPI = NT == 32 ? 1 : 2;
+  static constexpr int TOK = NT / EPI;
+  static constexpr int THREADS = 128 * (3 + EPI);
   static constexpr int B_COLS = NT * TERMS >= 128 ? 128 : 256;
   static constexpr int B_BYTES = NT * TERMS * B_COLS * 2;
   static constexpr int B_STAGES = 4;
@@ -127,6 +131,36 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// 16 columns of this warp's lanes, without waiting; and the wait, tied to the registers that it makes valid.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                 "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+// acc[i] += v[i] * f for 16 values, two to an instruction.
+__device__ __forceinline__ void fma16_scaled(float* acc, const float (&v)[16], float f) {
+  uint64_t ff;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(ff) : "f"(f));
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    uint64_t a, b;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc[i]), "f"(acc[i + 1]));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(v[i]), "f"(v[i + 1]));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(b), "l"(ff));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[i]), "=f"(acc[i + 1]) : "l"(a));
+  }
+}
+
 // Bounded wait of a converged warp, every lane for itself (each needs its own acquire); they agree on giving up. The
 // hardware suspends the lanes meanwhile: polling warps take issue slots and shared-memory cycles from the others.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int who) {
@@ -209,7 +243,7 @@ __device__ __forceinline__ WmUnit wm_unit(const WmCtrl* ctl, const WmArgs& p, in
 }
 
 template <typename T, int MODE, int NT, int G>
-__global__ void __launch_bounds__(WM_THREADS, 1)
+__global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS, 1)
     w4_mma_kernel(const __grid_constant__ WmMaps maps, const __grid_constant__ WmArgs p) {
   using W = typename std::conditional<MODE == WS_DOWN, __nv_bfloat16, T>::type;   // the operands' type
   constexpr int TERMS = MODE == WS_DOWN ? 2 : 1;
@@ -240,7 +274,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->d_full[i], 1);
-      mbar_init(&ctl->d_empty[i], 4);
+      mbar_init(&ctl->d_empty[i], 4 * S::EPI);
     }
     mbar_init(&ctl->mma_done, 1);
     ctl->abort_flag = 0;
@@ -280,7 +314,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
   };
 
   if (warp < 4) {
-    if constexpr (NT == 128) regs_dec<WM_REGS_CTRL>();
+    if constexpr (S::EPI == 2) regs_dec<WM_REGS_CTRL>();
     if (warp == 0 && elect_one()) {
       // ---------------- codes ----------------
       const uint64_t pol = policy_evict_first();
@@ -382,7 +416,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
     }
   } else if (warp < 12) {
     // ---------------- codes to numbers: the warpgroups take turns with the steps ----------------
-    if constexpr (NT == 128) regs_dec<WM_REGS_CONV>();
+    if constexpr (S::EPI == 2) regs_dec<WM_REGS_CONV>();
     const uint32_t wg = (warp - 4) >> 2;
     const int q4 = warp & 3;
     // Row of the shared tile behind this lane of tensor memory; `up` puts X1's 16 rows and X2's side by side.
@@ -441,9 +475,11 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
     }
   } else {
     // ---------------- scale and store ----------------
-    if constexpr (NT == 128) regs_inc<WM_REGS_EPI>();
-    const int q4 = warp & 3;
+    if constexpr (S::EPI == 2) regs_inc<WM_REGS_EPI>();
+    constexpr int TOK = S::TOK;
+    const int q4 = warp & 3, tok0 = (warp - 12) / 4 * TOK;               // this warpgroup's first token of a tile
     const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    const bool vec = groups % 8 == 0 && (reinterpret_cast<uintptr_t>(p.w.scale) & 15u) == 0;
     uint32_t d_it = 0;
     bool stop = false;
     for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
@@ -454,47 +490,72 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       const long long mrow = MODE == WS_UP ? static_cast<long long>(w.expert) * 2 * p.N + (lane >> 4) * static_cast<long long>(p.N) + min(col, p.N - 1)
                                            : static_cast<long long>(w.expert) * p.N + min(col, p.N - 1);
       const T* srow = static_cast<const T*>(p.w.scale) + mrow * groups;
-      // Scales of the next batch, in flight while this one is waited for; 0 past the last group.
-      auto scales = [&](int g, float (&f)[GPB]) {
+      // The row's scales, 8 at a time (one 16-byte load where the rows allow it) and 8 ahead; 0 past the last group.
+      auto load8 = [&](int g, uint32_t (&o)[4]) {
+        if (vec) {
+          const uint4 v = g < groups ? __ldg(reinterpret_cast<const uint4*>(srow + g)) : make_uint4(0, 0, 0, 0);
+          o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < GPB; ++i) f[i] = g + i < groups ? to_f32(srow[g + i]) : 0.0f;
+          for (int i = 0; i < 4; ++i) {
+            const T z = from_f32<T>(0.0f);
+            o[i] = pack2(g + 2 * i < groups ? srow[g + 2 * i] : z, g + 2 * i + 1 < groups ? srow[g + 2 * i + 1] : z);
+          }
+        }
       };
-      float total[NT];
+      uint32_t cur[4], nxt[4];
+      auto shift = [&]() {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) total[i] = 0.0f;
-      float next[GPB];
-      scales(s0 * GPS, next);
-      for (int g = s0 * GPS; g < s1 * GPS; g += GPB, ++d_it) {
-        float f[GPB];
+        for (int i = 0; i < 3; ++i) cur[i] = __funnelshift_r(cur[i], cur[i + 1], 16);
+        cur[3] >>= 16;
+      };
+      const int g_begin = s0 * GPS;
+      load8(g_begin & ~7, cur);
+      load8((g_begin & ~7) + 8, nxt);
+      for (int i = 0; i < (g_begin & 7); ++i) shift();
+      float total[TOK];
 #pragma unroll
-        for (int i = 0; i < GPB; ++i) f[i] = next[i];
-        scales(g + GPB, next);
+      for (int i = 0; i < TOK; ++i) total[i] = 0.0f;
+      for (int g = g_begin; g < s1 * GPS; g += GPB, ++d_it) {
         const uint32_t q = d_it & 1;
         if (!wait_warp(&ctl->d_full[q], (d_it >> 1) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { stop = true; break; }
         tc_fence_after();
+        const uint32_t src = tmem + lanes + q * S::D_COLS + tok0;
+        const int n = 16 << wm_box(w.tokens);
 #pragma unroll
-        for (int i = 0; i < GPB; ++i)
+        for (int i = 0; i < GPB; ++i) {
+          const uint16_t bits = static_cast<uint16_t>(cur[0]);
+          const float f = to_f32(*reinterpret_cast<const T*>(&bits));
+          shift();
+          if (((g + i) & 7) == 7) {
 #pragma unroll
-          for (int c = 0; c < NT / 32; ++c)
-            if (c * 32 < w.tokens) {
+            for (int j = 0; j < 4; ++j) cur[j] = nxt[j];
+            load8(g + i + 9, nxt);
+          }
+          // 16 columns at a time, the next 16 on their way while these are added.
+          float v[2][16];
+          tmem_ld16(src + i * NC, v[0]);
 #pragma unroll
-              for (int term = 0; term < TERMS; ++term) {
-                float v[32];
-                tmem_ld32(tmem + lanes + q * S::D_COLS + i * NC + term * (16 << wm_box(w.tokens)) + c * 32, v);
-                fma32_scaled(total + c * 32, v, f[i]);
-              }
-            }
+          for (int c = 0; c < TERMS * TOK / 16; ++c) {
+            tmem_wait_ld(v[c & 1]);
+            if (c + 1 < TERMS * TOK / 16)
+              tmem_ld16(src + i * NC + ((c + 1) % (TOK / 16)) * 16 + ((c + 1) / (TOK / 16)) * n, v[(c + 1) & 1]);
+            fma16_scaled(total + (c % (TOK / 16)) * 16, v[c & 1], f);
+          }
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->d_empty[q]);
       }
       if (stop) break;
+      const int tokens = w.tokens - tok0;                               // of this warpgroup
+      const long long row0 = w.row0 + tok0;
       if constexpr (MODE == WS_LINEAR) {
         if (col < p.N) {
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-            if (i < w.tokens) {
-              const long long at = static_cast<long long>(w.row0 + i) * p.N + col;
+          for (int i = 0; i < TOK; ++i)
+            if (i < tokens) {
+              const long long at = (row0 + i) * p.N + col;
               if (p.splits > 1)
                 p.y[static_cast<long long>(w.split) * p.M * p.N + at] = total[i];
               else
@@ -504,24 +565,24 @@ __global__ void __launch_bounds__(WM_THREADS, 1)
       } else if constexpr (MODE == WS_DOWN) {
         if (col < p.N) {
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-            if (i < w.tokens) p.y[static_cast<long long>(w.row0 + i) * p.N + col] = total[i];
+          for (int i = 0; i < TOK; ++i)
+            if (i < tokens) p.y[(row0 + i) * p.N + col] = total[i];
         }
       } else {
         // Lanes 0-15 hold X1, lanes 16-31 X2 of the same columns: even tokens end in the first, odd in the second.
         // hi + lo bf16 carry 16 bits of h; the columns go in pair order, zeros up to the next 64.
         const int pos = pair_pos(col), mine = lane >> 4;
 #pragma unroll
-        for (int i = 0; i < NT; i += 2)
-          if (i < w.tokens) {
+        for (int i = 0; i < TOK; i += 2)
+          if (i < tokens) {
             const float give = mine ? total[i] : total[i + 1];
             const float got = __shfl_xor_sync(0xffffffffu, give, 16);
             const float u1 = mine ? got : total[i], u2 = mine ? total[i + 1] : got;
             const float hv = col < p.N ? u1 * (u2 / (1.0f + expf(-u2))) : 0.0f;
-            if (i + mine < w.tokens) {
+            if (i + mine < tokens) {
               const __nv_bfloat16 hi = __float2bfloat16_rn(hv);
               const float rest = hv - __bfloat162float(hi);
-              const long long at = static_cast<long long>(w.row0 + i + mine) * p.h_pitch + pos;
+              const long long at = (row0 + i + mine) * p.h_pitch + pos;
               p.h[at] = hi;
               // An infinity or NaN has no remainder.
               p.h[static_cast<long long>(p.row_cap) * p.h_pitch + at] = __float2bfloat16_rn(fabsf(rest) <= 3.4e38f ? rest : 0.0f);
