@@ -157,10 +157,10 @@ int hidden_bf16_map(const void* hidden, int T, CUtensorMap* map) {
 // (programmatic dependent launch; GEMM1 allows it once all its CTAs are resident, GEMM2 waits per
 // tile on the readiness counters GEMM1 publishes).
 template <typename... KArgs, typename... Args>
-cudaError_t launch_programmatic(void (*kernel)(KArgs...), int grid, int block, int smem, cudaStream_t st,
-                                Args&&... args) {
+cudaError_t launch_programmatic_3d(void (*kernel)(KArgs...), dim3 grid, int block, int smem, cudaStream_t st,
+                                   Args&&... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(block));
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = st;
@@ -170,6 +170,12 @@ cudaError_t launch_programmatic(void (*kernel)(KArgs...), int grid, int block, i
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_programmatic(void (*kernel)(KArgs...), int grid, int block, int smem, cudaStream_t st,
+                                Args&&... args) {
+  return launch_programmatic_3d(kernel, dim3(static_cast<unsigned>(grid)), block, smem, st, std::forward<Args>(args)...);
 }
 
 cudaError_t launch_gemm2(const Gemm2Args& g2, int grid, cudaStream_t st) {
@@ -711,8 +717,7 @@ LinearW4Ws make_linear_w4_ws(int M, int N, int K) {
 }
 
 struct ExpertsW4Ws {
-  size_t h8;                                     // up to 8 tokens: fp32 [T k][T][I]
-  size_t counts, slot, x, h, y, c13, c2, total;  // more
+  size_t counts, slot, x, h, y, c13, c2, total;
 };
 ExpertsW4Ws make_experts_w4_ws(int T, int k, int E, int H, int I) {
   ExpertsW4Ws w{};
@@ -723,18 +728,14 @@ ExpertsW4Ws make_experts_w4_ws(int T, int k, int E, int H, int I) {
     return o;
   };
   const size_t routes = static_cast<size_t>(T) * k;
-  if (T <= WS_TOK) {
-    w.h8 = take(sizeof(float) * routes * T * I);
-  } else {
-    w.counts = take(sizeof(int) * E);
-    w.slot = take(sizeof(int) * routes);
-    w.x = take(routes * round_up(H, 64) * 2);
-    w.h = take(routes * round_up(I, 64) * 4);
-    w.y = take(routes * H * 4);
-    // Copies of codes whose rows do not allow TMA (odd widths).
-    w.c13 = take(w4_bytes(H) % 16 ? static_cast<size_t>(E) * 2 * I * round_up(w4_bytes(H), 16) : 0);
-    w.c2 = take(w4_bytes(I) % 16 ? static_cast<size_t>(E) * H * round_up(w4_bytes(I), 16) : 0);
-  }
+  w.counts = take(sizeof(int) * E);
+  w.slot = take(sizeof(int) * routes);
+  w.x = take(routes * round_up(H, 64) * 2);
+  w.h = take(routes * round_up(I, 64) * 4);
+  w.y = take(routes * H * 4);
+  // Copies of codes whose rows do not allow TMA (odd widths).
+  w.c13 = take(w4_bytes(H) % 16 ? static_cast<size_t>(E) * 2 * I * round_up(w4_bytes(H), 16) : 0);
+  w.c2 = take(w4_bytes(I) % 16 ? static_cast<size_t>(E) * H * round_up(w4_bytes(I), 16) : 0);
   w.total = off;
   return w;
 }
@@ -780,10 +781,10 @@ int wm_prepare(int smem, bool split_regs) {
 
 template <typename T, int MODE, int NT, int G>
 int launch_w4_mma_g(DeviceInfo* d, const WmMaps& maps, const WmArgs& a, long long units, cudaStream_t st) {
-  constexpr int smem = WM_SMEM<NT, MODE == WS_DOWN ? 2 : 1>;
+  constexpr int smem = WM_SMEM<NT, MODE == WS_DOWN ? 2 : 1, G>;
   if (int rc = wm_prepare<w4_mma_kernel<T, MODE, NT, G>>(smem, NT > 32)) return rc;
   const int grid = units < d->num_sms ? static_cast<int>(units) : d->num_sms;
-  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT, G>, grid < 1 ? 1 : grid, WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS, smem, st, maps, a),
+  return cuda_check(launch_programmatic(w4_mma_kernel<T, MODE, NT, G>, grid < 1 ? 1 : grid, WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREADS, smem, st, maps, a),
                     "w4_mma launch");
 }
 
@@ -799,10 +800,10 @@ int launch_w4_mma_nt(DeviceInfo* d, const WmArgs& a, const void* x, long long x_
     if (int rc = w4_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w.codes, dims, strides, box, &maps.codes)) return rc;
   }
   const CUtensorMapDataType t = MODE != WS_DOWN && std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  for (int i = 0; i < 4 && (16 << i) <= NT; ++i) {
+  for (int i = 0; 16 * (i + 1) <= NT; ++i) {
     const long long pitch = round_up(a.K, 64) * 2ll, rows = x_rows / TERMS;
     const long long dims[4] = {64, rows, TERMS, pitch / 128}, strides[3] = {pitch, pitch * rows, 128};
-    const int box[4] = {64, 16 << i, TERMS, WmShape<NT, TERMS>::B_COLS / 64};
+    const int box[4] = {64, 16 * (i + 1), TERMS, WmShape<NT, TERMS, 128>::B_COLS / 64};
     if (int rc = w4_map(t, x, dims, strides, box, &maps.x[i])) return rc;
   }
   const int per = MODE == WS_UP ? 64 : 128;
@@ -855,7 +856,7 @@ int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Mat
   WmArgs a{};
   a.w = w;
   if (int rc = w4_tma_codes(d, w.codes, N, K, W + ws.codes, &a.w.codes, st)) return rc;
-  pair_rows_kernel<T><<<grid_for(static_cast<size_t>(M) * (round_up(K, 64) / 8), 256, d->num_sms * 8), 256, 0, st>>>(
+  pair_rows_kernel<T><<<dim3((round_up(K, 64) / 8 + 255) / 256, M), 256, 0, st>>>(
       static_cast<const T*>(x), x_stride, M, K, reinterpret_cast<T*>(W + ws.x));
   a.E = 1;
   a.N = N;
@@ -881,27 +882,6 @@ int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Mat
 template <typename T>
 int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W, cudaStream_t st) {
   const ExpertsW4Ws ws = make_experts_w4_ws(p.T, p.k, p.E, p.H, p.I);
-  if (p.T <= WS_TOK) {
-    float* h = reinterpret_cast<float*>(W + ws.h8);
-    auto split = [&](StreamArgs& b, int at_least) {
-      const int steps = (b.K + WS_STEP - 1) / WS_STEP, need_parts = (steps + WS_CHUNK - 1) / WS_CHUNK;
-      b.parts = at_least > need_parts ? at_least : need_parts;
-      if (b.parts > steps) b.parts = steps;
-      b.spp = (steps + b.parts - 1) / b.parts;
-      b.parts = (steps + b.spp - 1) / b.spp;
-    };
-    // First product: the columns of a pick's expert over a cluster, at most 16 steps per block.
-    StreamArgs up{p.x, p.x_stride, p.w13, p.T, p.I, p.H, 1, 0, 0, p.idx, p.wt, p.k, p.E, p.offset, h, nullptr};
-    const int steps = (p.H + WS_STEP - 1) / WS_STEP;
-    int cluster = 1;
-    while (cluster < 8 && steps > WS_CHUNK * cluster) cluster *= 2;
-    split(up, cluster);
-    // Second product: the active experts' columns over a cluster of 8.
-    StreamArgs down{nullptr, 0, p.w2, p.T, p.H, p.I, 1, 0, 0, p.idx, p.wt, p.k, p.E, p.offset, h, out};
-    split(down, 1);
-    if (int rc = cuda_check(launch_w4_stream<T, WS_UP>(up, cluster, p.T * p.k, false, st), "experts_w4 first product")) return rc;
-    return cuda_check(launch_w4_stream<T, WS_DOWN>(down, 8, 1, true, st), "experts_w4 second product");
-  }
   const int routes = p.T * p.k;
   int* counts = reinterpret_cast<int*>(W + ws.counts);
   int* slot = reinterpret_cast<int*>(W + ws.slot);
@@ -913,10 +893,14 @@ int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W
   down.w = p.w2;
   if (int rc = w4_tma_codes(d, p.w13.codes, 2ll * p.E * p.I, p.H, W + ws.c13, &up.w.codes, st)) return rc;
   if (int rc = w4_tma_codes(d, p.w2.codes, static_cast<long long>(p.E) * p.H, p.I, W + ws.c2, &down.w.codes, st)) return rc;
-  if (int rc = cuda_check(cudaMemsetAsync(counts, 0, sizeof(int) * p.E, st), "memset counts")) return rc;
-  experts_slot_kernel<<<grid_for(static_cast<size_t>(routes), 256, d->num_sms * 4), 256, 0, st>>>(p.idx, routes, p.offset, p.E, counts, slot);
-  experts_gather_kernel<T><<<grid_for(static_cast<size_t>(routes), 8, d->num_sms * 8), 256, 0, st>>>(
-      static_cast<const T*>(p.x), p.x_stride, p.idx, routes, p.k, p.offset, p.E, counts, p.H, slot, xg);
+  if (routes <= WM_PLAN_MAX) {
+    experts_plan_kernel<T><<<routes, 256, 0, st>>>(static_cast<const T*>(p.x), p.x_stride, p.idx, routes, p.k, p.offset, p.E, p.H, counts, slot, xg);
+  } else {
+    if (int rc = cuda_check(cudaMemsetAsync(counts, 0, sizeof(int) * p.E, st), "memset counts")) return rc;
+    experts_slot_kernel<<<grid_for(static_cast<size_t>(routes), 256, d->num_sms * 4), 256, 0, st>>>(p.idx, routes, p.offset, p.E, counts, slot);
+    experts_gather_kernel<T><<<grid_for(static_cast<size_t>(routes), 8, d->num_sms * 8), 256, 0, st>>>(
+        static_cast<const T*>(p.x), p.x_stride, p.idx, routes, p.k, p.offset, p.E, counts, p.H, slot, xg);
+  }
   up.E = down.E = p.E;
   up.counts = down.counts = counts;
   up.row_cap = down.row_cap = routes;
@@ -931,9 +915,9 @@ int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W
   const int tile = wm_tile((routes + p.E - 1) / p.E);
   if (int rc = launch_w4_mma<T, WS_UP>(d, up, xg, routes, tile, st)) return rc;
   if (int rc = launch_w4_mma<T, WS_DOWN>(d, down, h, 2ll * routes, tile, st)) return rc;
-  return cuda_check(launch_programmatic(experts_combine_kernel<T>, grid_for(static_cast<size_t>(p.T) * p.H, 256, d->num_sms * 16), 256, 0, st,
-                                        static_cast<const float*>(y), static_cast<const int*>(slot), p.wt, p.T, p.k, p.H,
-                                        static_cast<T*>(out)),
+  const int vec = p.H % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
+  return cuda_check(launch_programmatic_3d(experts_combine_kernel<T>, dim3((p.H + 1023) / 1024, p.T), 256, 0, st, static_cast<const float*>(y),
+                                           static_cast<const int*>(slot), p.wt, p.k, p.H, vec, static_cast<T*>(out)),
                     "experts_combine launch");
 }
 

@@ -31,9 +31,9 @@ constexpr int WM_LAUNCH_REGS_MIN = (WM_REGS_CTRL + 2 * WM_REGS_CONV + 2 * WM_REG
 // Shared memory: a ring of steps of codes, a ring of token rows. An entry of the second holds B_COLS columns of every
 // term (up to 64 KB), so that a step of few tokens is one entry.
 // Tensor memory: two batches of accumulators, then the weights of as many steps (128 columns each) as fit.
-template <int NT, int TERMS>
+template <int NT, int TERMS, int G>
 struct WmShape {
-  static constexpr int D_COLS = NT * TERMS >= 128 ? 128 : 64;
+  static constexpr int D_COLS = NT * TERMS * (WM_STEP / G) >= 128 ? 128 : NT * TERMS * (WM_STEP / G);
   static constexpr int A_COL = 2 * D_COLS;
   static constexpr int A_SLOTS = (512 - A_COL) / 128;
   // Warpgroups that scale, each TOK tokens of the tile: above 32 tokens one would be the slowest of the roles.
@@ -60,15 +60,15 @@ struct WmCtrl {
   int row_off[RX_MAX_E + 1];                    // first row of each expert in the route-ordered buffers
 };
 
-template <int NT, int TERMS>
-constexpr int WM_SMEM = WmShape<NT, TERMS>::RING + static_cast<int>(sizeof(WmCtrl)) + 1024;
+template <int NT, int TERMS, int G>
+constexpr int WM_SMEM = WmShape<NT, TERMS, G>::RING + static_cast<int>(sizeof(WmCtrl)) + 1024;
 
 // Tensor maps. codes: 4-D (bytes of a row, rows, X1 / X2, experts), one box per step. x: 4-D (64 columns, rows, terms,
-// blocks of 64 columns), one map for each box height of 16, 32, 64, 128 rows; a box is a ring entry as the mma reads it.
+// blocks of 64 columns), one map for each box height of 16, 32, ... 128 rows; a box is a ring entry as the mma reads it.
 // One copy instruction per entry: a producer's thread needs some hundred cycles for each.
 struct WmMaps {
   CUtensorMap codes;
-  CUtensorMap x[4];
+  CUtensorMap x[8];
 };
 
 struct WmArgs {
@@ -213,8 +213,8 @@ __device__ __forceinline__ void wm_build_map(int* tile_off, int* row_off, const 
   }
 }
 
-// Operand columns of a tile's tokens, 16 << wm_box(tokens): the height of the box that brings them.
-__device__ __forceinline__ int wm_box(int tokens) { return (tokens > 16) + (tokens > 32) + (tokens > 64); }
+// Operand columns of a tile's tokens: the height of the box that brings them.
+__device__ __forceinline__ int wm_cols(int tokens) { return (tokens + 15) & ~15; }
 
 struct WmUnit {
   int expert, row0, tokens;    // first row and count of the tile's tokens
@@ -243,11 +243,11 @@ __device__ __forceinline__ WmUnit wm_unit(const WmCtrl* ctl, const WmArgs& p, in
 }
 
 template <typename T, int MODE, int NT, int G>
-__global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS, 1)
+__global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREADS, 1)
     w4_mma_kernel(const __grid_constant__ WmMaps maps, const __grid_constant__ WmArgs p) {
   using W = typename std::conditional<MODE == WS_DOWN, __nv_bfloat16, T>::type;   // the operands' type
   constexpr int TERMS = MODE == WS_DOWN ? 2 : 1;
-  using S = WmShape<NT, TERMS>;
+  using S = WmShape<NT, TERMS, G>;
   constexpr int GPS = WM_STEP / G;                                      // groups per step
   constexpr int NC = NT * TERMS;                                        // columns of one accumulator
   constexpr int GPB = S::D_COLS / NC < GPS ? S::D_COLS / NC : GPS;      // groups per batch of accumulators
@@ -343,9 +343,9 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS,
         const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
         int s0, s1;
         range(w, s0, s1);
-        const int box = wm_box(w.tokens);                    // rows past the tile's are read for nothing
-        const CUtensorMap* map = &maps.x[box];
-        const uint32_t bytes = (16u << box) * S::B_COLS * 2 * TERMS;
+        const int n = wm_cols(w.tokens);                     // rows past the tile's are read for nothing
+        const CUtensorMap* map = &maps.x[n / 16 - 1];
+        const uint32_t bytes = n * S::B_COLS * 2 * TERMS;
         for (int c = s0 * ENTRIES; c < s1 * ENTRIES; ++c, ++it) {
           const int st = it % S::B_STAGES;
           if (!mbar_wait(&ctl->b_empty[st], ((it / S::B_STAGES) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_PRODUCER)) break;
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS,
         const WmUnit w = wm_unit<NT>(ctl, p, u, row_tiles);
         int s0, s1;
         range(w, s0, s1);
-        const int n = TERMS * (16 << wm_box(w.tokens));
+        const int n = TERMS * wm_cols(w.tokens);
         const uint64_t chunk = static_cast<uint64_t>(n * 128 >> 4);    // from one block of 64 columns to the next
         constexpr uint32_t fmt = std::is_same_v<W, __half> ? 0u : (1u << 7) | (1u << 10);
         const uint32_t idesc = (1u << 4) | fmt | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS,
         if (!wait_warp(&ctl->d_full[q], (d_it >> 1) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) { stop = true; break; }
         tc_fence_after();
         const uint32_t src = tmem + lanes + q * S::D_COLS + tok0;
-        const int n = 16 << wm_box(w.tokens);
+        const int n = wm_cols(w.tokens);
 #pragma unroll
         for (int i = 0; i < GPB; ++i) {
           const uint16_t bits = static_cast<uint16_t>(cur[0]);
@@ -536,11 +536,15 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1>::THREADS,
           float v[2][16];
           tmem_ld16(src + i * NC, v[0]);
 #pragma unroll
-          for (int c = 0; c < TERMS * TOK / 16; ++c) {
-            tmem_wait_ld(v[c & 1]);
-            if (c + 1 < TERMS * TOK / 16)
-              tmem_ld16(src + i * NC + ((c + 1) % (TOK / 16)) * 16 + ((c + 1) / (TOK / 16)) * n, v[(c + 1) & 1]);
-            fma16_scaled(total + (c % (TOK / 16)) * 16, v[c & 1], f);
+          for (int c = 0; c < TERMS * (TOK / 16); ++c) {
+            // Piece c: 16 tokens of one term, the terms of a token side by side. Pieces past the tile's tokens hold nothing;
+            // leaving them out pays for small tiles only (it breaks the overlap of loads and sums).
+            const int ahead = (c + 1) / TERMS * 16 + (c + 1) % TERMS * n;
+            if (NT > 32 || c / TERMS * 16 < n) {
+              tmem_wait_ld(v[c & 1]);
+              if (c + 1 < TERMS * (TOK / 16) && (NT > 32 || (c + 1) / TERMS * 16 < n)) tmem_ld16(src + i * NC + ahead, v[(c + 1) & 1]);
+              fma16_scaled(total + c / TERMS * 16, v[c & 1], f);
+            }
           }
         }
         tc_fence_before();
@@ -615,17 +619,14 @@ __device__ __forceinline__ uint4 ld_pairs(const T* row, int k, int K) {
   return *reinterpret_cast<const uint4*>(o);
 }
 
-// Rows of x in pair order, columns padded with zeros to a multiple of 64.
+// Rows of x in pair order, columns padded with zeros to a multiple of 64. One warp per row and stretch of columns.
 template <typename T>
 __global__ void __launch_bounds__(256) pair_rows_kernel(const T* x, long long x_stride, int M, int K, T* out) {
   allow_dependent_launch();
   const int per = (K + 63) / 64 * 8;
-  const long long n = static_cast<long long>(M) * per;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const long long m = i / per;
-    const int c = static_cast<int>(i % per);
-    reinterpret_cast<uint4*>(out)[i] = ld_pairs(x + m * x_stride, c * 8, K);
-  }
+  const long long m = blockIdx.y;
+  for (int c = blockIdx.x * 256 + threadIdx.x; c < per; c += gridDim.x * 256)
+    reinterpret_cast<uint4*>(out)[m * per + c] = ld_pairs(x + m * x_stride, c * 8, K);
 }
 
 // Codes with a row pitch of a multiple of 16 bytes, for shapes whose own rows do not allow TMA.
@@ -649,6 +650,58 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const float* y, int spli
     for (int s = 1; s < splits; ++s) v += y[s * n + i];
     out[i] = from_f32<T>(v);
   }
+}
+
+// Rows of up to 64 KB or so, 16 bytes per lane and step: four in flight per lane.
+template <typename T>
+__device__ __forceinline__ void copy_row_pairs(const T* row, int K, uint4* out, int first, int stride) {
+  const int per = (K + 63) / 64 * 8;
+  int c = first;
+  for (; c + 3 * stride < per; c += 4 * stride) {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ld_pairs(row, (c + i * stride) * 8, K);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[c + i * stride] = v[i];
+  }
+  for (; c < per; c += stride) out[c] = ld_pairs(row, c * 8, K);
+}
+
+constexpr int WM_PLAN_MAX = 1024;   // picks that the one-kernel plan handles
+
+// Few picks: one block per pick finds its row's place by itself (experts in order, picks of an expert in order) and
+// copies the row; block 0 also counts the experts' picks. place[r]: the pick's row, or -1.
+template <typename T>
+__global__ void __launch_bounds__(256) experts_plan_kernel(const T* x, long long x_stride, const int* idx, int n, int k, int offset, int E,
+                                                           int H, int* counts, int* place, T* out) {
+  __shared__ int hist[RX_MAX_E];
+  allow_dependent_launch();
+  const int r = blockIdx.x, id = idx[r], e = id >= offset && id - offset < E ? id - offset : -1;
+  int before = 0;
+  if (r == 0) {
+    for (int i = threadIdx.x; i < E; i += 256) hist[i] = 0;
+    __syncthreads();
+  }
+  for (int q = threadIdx.x; q < n; q += 256) {
+    const int iq = idx[q], eq = iq >= offset && iq - offset < E ? iq - offset : -1;
+    if (eq < 0) continue;
+    before += eq < e || (eq == e && q < r) ? 1 : 0;
+    if (r == 0) atomicAdd(&hist[eq], 1);
+  }
+  __shared__ int warp_sum_[8];
+  before = __reduce_add_sync(0xffffffffu, before);
+  if ((threadIdx.x & 31) == 0) warp_sum_[threadIdx.x >> 5] = before;
+  __syncthreads();
+  if (r == 0)
+    for (int i = threadIdx.x; i < E; i += 256) counts[i] = hist[i];
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) at += warp_sum_[i];
+  if (threadIdx.x == 0) place[r] = e < 0 ? -1 : at;
+  if (e < 0) return;
+  const int per = (H + 63) / 64 * 8;
+  copy_row_pairs(x + static_cast<long long>(r / k) * x_stride, H, reinterpret_cast<uint4*>(out) + static_cast<long long>(at) * per,
+                 static_cast<int>(threadIdx.x), 256);
 }
 
 // Each local pick takes a place in its expert's list. The order within a list changes from call to call and no
@@ -678,27 +731,53 @@ __global__ void __launch_bounds__(256) experts_gather_kernel(const T* x, long lo
       if (lane == 0) report_status(ST_BAD_INDEX);
       continue;
     }
-    const T* row = x + static_cast<long long>(r / k) * x_stride;
-    for (int c = lane; c < per; c += 32) reinterpret_cast<uint4*>(out)[static_cast<long long>(at) * per + c] = ld_pairs(row, c * 8, H);
+    copy_row_pairs(x + static_cast<long long>(r / k) * x_stride, H, reinterpret_cast<uint4*>(out) + static_cast<long long>(at) * per, lane, 32);
     __syncwarp();
     if (lane == 0) slot[r] = at;
   }
 }
 
-// out[t] = sum over the token's local picks, in their order, of weight * y[row], rounded once.
+// out[t] = sum over the token's local picks, in their order, of weight * y[row], rounded once. Blocks of 1024 columns
+// of a token; `vec`: 4 neighbouring columns per thread (H a multiple of 4, out 8-byte aligned).
 template <typename T>
-__global__ void __launch_bounds__(256) experts_combine_kernel(const float* y, const int* place, const float* wt, int T_, int k, int H, T* out) {
+__global__ void __launch_bounds__(256) experts_combine_kernel(const float* y, const int* place, const float* wt, int k, int H, int vec, T* out) {
+  __shared__ int row[RX_MAX_K];
+  __shared__ float weight[RX_MAX_K];
+  __shared__ int count;
+  const long long t = blockIdx.y;
   wait_prerequisite_grids();
-  const long long n = static_cast<long long>(T_) * H;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const long long t = i / H;
-    const int c = static_cast<int>(i % H);
-    float acc = 0.0f;
-    for (int j = 0; j < k; ++j) {
-      const int r = place[t * k + j];
-      if (r >= 0) acc = fmaf(wt[t * k + j], y[static_cast<long long>(r) * H + c], acc);
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    const int r = lane < k ? place[t * k + lane] : -1;
+    const uint32_t m = __ballot_sync(0xffffffffu, r >= 0);
+    if (r >= 0) {
+      const int at = __popc(m & ((1u << lane) - 1u));
+      row[at] = r;
+      weight[at] = wt[t * k + lane];
     }
-    out[i] = from_f32<T>(acc);
+    if (lane == 0) count = __popc(m);
+  }
+  __syncthreads();
+  const int n = count, c = blockIdx.x * 1024 + threadIdx.x * (vec ? 4 : 1);
+  if (vec) {
+    if (c >= H) return;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j = 0; j < n; ++j) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(y + static_cast<long long>(row[j]) * H + c));
+      const float w = weight[j];
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
+    }
+    *reinterpret_cast<uint2*>(out + t * H + c) =
+        make_uint2(pack2(from_f32<T>(acc.x), from_f32<T>(acc.y)), pack2(from_f32<T>(acc.z), from_f32<T>(acc.w)));
+  } else {
+    for (int i = c; i < min(H, static_cast<int>(blockIdx.x + 1) * 1024); i += 256) {
+      float acc = 0.0f;
+      for (int j = 0; j < n; ++j) acc = fmaf(weight[j], y[static_cast<long long>(row[j]) * H + i], acc);
+      out[t * H + i] = from_f32<T>(acc);
+    }
   }
 }
 
