@@ -898,7 +898,7 @@ int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W
   } else {
     if (int rc = cuda_check(cudaMemsetAsync(counts, 0, sizeof(int) * p.E, st), "memset counts")) return rc;
     experts_slot_kernel<<<grid_for(static_cast<size_t>(routes), 256, d->num_sms * 4), 256, 0, st>>>(p.idx, routes, p.offset, p.E, counts, slot);
-    experts_gather_kernel<T><<<grid_for(static_cast<size_t>(routes), 8, d->num_sms * 8), 256, 0, st>>>(
+    experts_gather_kernel<T><<<grid_for(static_cast<size_t>(routes), WM_GATHER, d->num_sms * 16), 256, 0, st>>>(
         static_cast<const T*>(p.x), p.x_stride, p.idx, routes, p.k, p.offset, p.E, counts, p.H, slot, xg);
   }
   up.E = down.E = p.E;

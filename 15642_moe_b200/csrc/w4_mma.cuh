@@ -31,6 +31,9 @@ constexpr int WM_LAUNCH_REGS_MIN = (WM_REGS_CTRL + 2 * WM_REGS_CONV + 2 * WM_REG
 // Shared memory: a ring of steps of codes, a ring of token rows. An entry of the second holds B_COLS columns of every
 // term (up to 64 KB), so that a step of few tokens is one entry.
 // Tensor memory: two batches of accumulators, then the weights of as many steps (128 columns each) as fit.
+// A barrier's parity tells only neighbouring uses apart. The converting warpgroups take every second step, so they skip uses
+// of a ring whose length is odd; that is safe here because the mma of the steps before them has finished by then (the weights'
+// slots are fewer than the codes' stages and are given back in order).
 template <int NT, int TERMS, int G>
 struct WmShape {
   static constexpr int D_COLS = NT * TERMS * (WM_STEP / G) >= 128 ? 128 : NT * TERMS * (WM_STEP / G);
@@ -436,8 +439,9 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
             : static_cast<long long>(w.expert) * p.N + min(w.rt * 128 + srow, p.N - 1);
         zrow = p.w.zero + r * groups;
       }
-      for (int s = s0; s < s1 && ok; ++s, ++it) {
-        if ((it & 1u) != wg) continue;
+      const uint32_t end = it + static_cast<uint32_t>(s1 - s0);
+      int s = s0 + static_cast<int>((it ^ wg) & 1u);                   // the warpgroups take turns across units
+      for (it += (it ^ wg) & 1u; it < end; it += 2, s += 2) {
         const uint32_t st = it % S::CODE_STAGES, slot = it % S::A_SLOTS;
         uint32_t off[GPS];
 #pragma unroll
@@ -472,6 +476,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->a_full[slot]);
       }
+      it = end;
     }
   } else {
     // ---------------- scale and store ----------------
@@ -668,6 +673,7 @@ __device__ __forceinline__ void copy_row_pairs(const T* row, int K, uint4* out, 
 }
 
 constexpr int WM_PLAN_MAX = 1024;   // picks that the one-kernel plan handles
+constexpr int WM_GATHER = 16;       // picks that a block of the gather looks at together
 
 // Few picks: one block per pick finds its row's place by itself (experts in order, picks of an expert in order) and
 // copies the row; block 0 also counts the experts' picks. place[r]: the pick's row, or -1.
@@ -722,18 +728,29 @@ __global__ void __launch_bounds__(256) experts_gather_kernel(const T* x, long lo
   allow_dependent_launch();
   if (threadIdx.x < 32) wm_build_map(tile_off, row_off, counts, E, n, 128);
   __syncthreads();
-  const int per = (H + 63) / 64 * 8, lane = threadIdx.x & 31;
-  for (int r = (blockIdx.x * 256 + threadIdx.x) >> 5; r < n; r += gridDim.x * 8) {
-    const int s = slot[r];
-    if (s < 0) continue;
-    const int at = row_off[idx[r] - offset] + s;
-    if (at >= n) {
-      if (lane == 0) report_status(ST_BAD_INDEX);
-      continue;
+  // A block looks at some picks at a time, then copies the local ones' rows together.
+  __shared__ int place[WM_GATHER];
+  const int per = (H + 63) / 64 * 8;
+  for (int base = blockIdx.x * WM_GATHER; base < n; base += gridDim.x * WM_GATHER) {
+    __syncthreads();
+    if (threadIdx.x < WM_GATHER) {
+      const int r = base + static_cast<int>(threadIdx.x);
+      int at = -1;
+      if (r < n && slot[r] >= 0) {
+        at = row_off[idx[r] - offset] + slot[r];
+        if (at >= n) {
+          report_status(ST_BAD_INDEX);
+          at = -1;
+        }
+        slot[r] = at;
+      }
+      place[threadIdx.x] = at;
     }
-    copy_row_pairs(x + static_cast<long long>(r / k) * x_stride, H, reinterpret_cast<uint4*>(out) + static_cast<long long>(at) * per, lane, 32);
-    __syncwarp();
-    if (lane == 0) slot[r] = at;
+    __syncthreads();
+    for (int i = 0; i < WM_GATHER; ++i)
+      if (place[i] >= 0)
+        copy_row_pairs(x + static_cast<long long>((base + i) / k) * x_stride, H, reinterpret_cast<uint4*>(out) + static_cast<long long>(place[i]) * per,
+                       static_cast<int>(threadIdx.x), 256);
   }
 }
 
