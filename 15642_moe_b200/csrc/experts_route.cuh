@@ -97,27 +97,27 @@ __device__ __forceinline__ void load_row(const T* row, int first, int E, bool ve
   }
 }
 
-__device__ __forceinline__ float sigmoid_f32(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
+// Scores for the choice: e^x by the hardware's 2^x (relative error below 2^-21 for logits of any size that matter). The
+// weights use expf.
+__device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
-// Key of a pick: larger pick, larger key; 0 for -inf (never chosen), the largest for NaN (it is chosen and
-// its weight shows it). x + 0 makes -0 and +0 equal.
+// Key of a pick: larger pick, larger key. x + 0 makes -0 and +0 equal and every NaN the positive one, the largest key:
+// a NaN is chosen and its weight shows it.
 __device__ __forceinline__ uint32_t pick_key(float x) {
-  if (x != x) return 0xFFFFFFFFu;
-  if (x == -INFINITY) return 0u;
-  return order_key(x + 0.0f);
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
+constexpr uint32_t RX_NONE = 0x007FFFFFu;       // the key of -inf: never chosen
 
 __device__ __forceinline__ float key_value(uint32_t key) {
-  if (key == 0u) return -INFINITY;
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
 
 template <typename T, int VPT>
 __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __grid_constant__ RouteExpertsArgs p) {
   extern __shared__ uint32_t rx_dyn[];                    // per warp: E pick keys, n_group group keys (grouped only)
-  __shared__ uint32_t cand_key[RX_WARPS][32];
-  __shared__ int cand_idx[RX_WARPS][32];
-  __shared__ float cand_s[RX_WARPS][32];
+  __shared__ uint2 cand[RX_WARPS][32];                    // key, expert
+  __shared__ float cand_x[RX_WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long t = static_cast<long long>(blockIdx.x) * RX_WARPS + warp;
   if (t >= p.T) return;
@@ -136,61 +136,93 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     mx = warp_max(mx);
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) sum += expf(x[i] - mx);
+    for (int i = 0; i < VPT; ++i) sum += __expf(x[i] - mx);
     inv = 1.0f / warp_sum(sum);
   }
-  auto score = [&](float l) { return p.softmax ? expf(l - mx) * inv : sigmoid_f32(l); };
   const bool grouped = p.n_group > 1;
   const bool by_logit = p.bias == nullptr && !(grouped && p.group_top2);
 
   uint32_t key[VPT];
+  if (by_logit) {
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int e = first + i;
-    float v = x[i];
-    if (!by_logit && v != -INFINITY) {
-      v = score(v);
-      if (p.bias != nullptr && e < p.E) v = __fadd_rn(v, __ldg(p.bias + e));
+    for (int i = 0; i < VPT; ++i) key[i] = pick_key(x[i]);            // -inf past E
+  } else {
+    float b[VPT];
+    if (p.bias != nullptr) {
+      load_row<float, VPT>(p.bias, first, p.E, p.E == 32 * VPT && (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0, 0.0f, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) b[i] = 0.0f;
     }
-    key[i] = e < p.E ? pick_key(v) : 0u;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const float v = __fadd_rn(p.softmax ? __expf(x[i] - mx) * inv : sigmoid_fast(x[i]), b[i]);
+      key[i] = x[i] == -INFINITY ? RX_NONE : pick_key(v);
+    }
   }
 
   if (grouped) {
-    const int per = p.E / p.n_group;
-    uint32_t* pk = rx_dyn + warp * (p.E + p.n_group);
-    uint32_t* gs = pk + p.E;
+    const int per = p.E / p.n_group, lanes = per / VPT;               // lanes of a group, where it is made of whole lanes
+    if (p.E == 32 * VPT && lanes >= 1 && (lanes & (lanes - 1)) == 0) {
+      // Two best of the lane's keys, then of the group's lanes.
+      uint32_t k1 = RX_NONE, k2 = RX_NONE;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (first + i < p.E) pk[first + i] = key[i];
-    __syncwarp();
-    uint32_t mine = 0u;                                   // key of group `lane`'s score
-    bool drop = false;
-    if (lane < p.n_group) {
-      uint32_t k1 = 0u, k2 = 0u;
-      for (int j = 0; j < per; ++j) {
-        const uint32_t v = pk[lane * per + j];
-        k2 = max(k2, min(k1, v));
-        k1 = max(k1, v);
+      for (int i = 0; i < VPT; ++i) {
+        k2 = max(k2, min(k1, key[i]));
+        k1 = max(k1, key[i]);
       }
-      mine = p.group_top2 ? pick_key(__fadd_rn(key_value(k1), key_value(k2))) : k1;
-      gs[lane] = mine;
-    }
-    __syncwarp();
-    if (lane < p.n_group) {
+      for (int o = 1; o < lanes; o <<= 1) {
+        const uint32_t o1 = __shfl_xor_sync(0xffffffffu, k1, o), o2 = __shfl_xor_sync(0xffffffffu, k2, o);
+        k2 = max(max(k2, o2), min(k1, o1));
+        k1 = max(k1, o1);
+      }
+      const uint32_t mine = p.group_top2 ? pick_key(__fadd_rn(key_value(k1), key_value(k2))) : k1;
       int rank = 0;
       for (int o = 0; o < p.n_group; ++o) {
-        const uint32_t other = gs[o];
-        rank += (other > mine || (other == mine && o < lane)) ? 1 : 0;
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, o * lanes);
+        rank += (other > mine || (other == mine && o * lanes < (lane & ~(lanes - 1)))) ? 1 : 0;
       }
-      drop = rank >= p.topk_group;
-    }
-    const uint32_t dropped = __ballot_sync(0xffffffffu, drop);
+      if (rank >= p.topk_group) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (first + i < p.E && ((dropped >> ((first + i) / per)) & 1u)) key[i] = 0u;
+        for (int i = 0; i < VPT; ++i) key[i] = RX_NONE;
+      }
+    } else {
+      uint32_t* pk = rx_dyn + warp * (p.E + p.n_group);
+      uint32_t* gs = pk + p.E;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (first + i < p.E) pk[first + i] = key[i];
+      __syncwarp();
+      uint32_t mine = RX_NONE;                            // key of group `lane`'s score
+      bool drop = false;
+      if (lane < p.n_group) {
+        uint32_t k1 = RX_NONE, k2 = RX_NONE;
+#pragma unroll 4
+        for (int j = 0; j < per; ++j) {
+          const uint32_t v = pk[lane * per + j];
+          k2 = max(k2, min(k1, v));
+          k1 = max(k1, v);
+        }
+        mine = p.group_top2 ? pick_key(__fadd_rn(key_value(k1), key_value(k2))) : k1;
+        gs[lane] = mine;
+      }
+      __syncwarp();
+      if (lane < p.n_group) {
+        int rank = 0;
+        for (int o = 0; o < p.n_group; ++o) {
+          const uint32_t other = gs[o];
+          rank += (other > mine || (other == mine && o < lane)) ? 1 : 0;
+        }
+        drop = rank >= p.topk_group;
+      }
+      const uint32_t dropped = __ballot_sync(0xffffffffu, drop);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (first + i < p.E && ((dropped >> ((first + i) / per)) & 1u)) key[i] = RX_NONE;
+    }
   }
 
-  // 1. A key that at least k experts reach (1 if fewer are left).
+  // 1. A key that at least k experts reach (or all that are left).
   uint32_t best = key[0];
 #pragma unroll
   for (int i = 1; i < VPT; ++i) best = max(best, key[i]);
@@ -199,7 +231,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     floor_key = __reduce_max_sync(0xffffffffu, left);
     if (left == floor_key) left = 0u;
   }
-  floor_key = max(floor_key, 1u);
+  floor_key = max(floor_key, RX_NONE + 1u);
 
   // 2. The experts that reach it, one per lane.
   int count = 0;
@@ -209,9 +241,8 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     const uint32_t m = __ballot_sync(0xffffffffu, in);
     const int at = count + __popc(m & ((1u << lane) - 1u));
     if (in && at < 32) {
-      cand_key[warp][at] = key[i];
-      cand_idx[warp][at] = first + i;
-      cand_s[warp][at] = x[i];
+      cand[warp][at] = make_uint2(key[i], static_cast<uint32_t>(first + i));
+      cand_x[warp][at] = x[i];
     }
     count += __popc(m);
   }
@@ -221,18 +252,17 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
   float my_x = 0.0f;
   if (count <= 32) {
     // 3. Rank among the candidates.
-    const uint32_t ck = lane < count ? cand_key[warp][lane] : 0u;
-    const int ci = lane < count ? cand_idx[warp][lane] : RX_MAX_E;
+    const uint2 mine = lane < count ? cand[warp][lane] : make_uint2(0u, RX_MAX_E);
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < count; ++j) {
-      const uint32_t ok = cand_key[warp][j];
-      const int oi = cand_idx[warp][j];
-      rank += (ok > ck || (ok == ck && oi < ci)) ? 1 : 0;
+      const uint2 o = cand[warp][j];
+      rank += (o.x > mine.x || (o.x == mine.x && o.y < mine.y)) ? 1 : 0;
     }
     if (lane < count && rank < p.k) {
       place = rank;
-      my_idx = ci;
-      my_x = cand_s[warp][lane];
+      my_idx = static_cast<int>(mine.y);
+      my_x = cand_x[warp][lane];
     }
     // Lanes past the candidates take the places that no expert fills.
     if (lane >= count && lane < p.k) place = lane;
@@ -247,7 +277,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
           bi = i;
         }
       const uint32_t mk = __reduce_max_sync(0xffffffffu, bk);
-      if (mk == 0u) {                                   // none left
+      if (mk <= RX_NONE) {                              // none left
         if (lane == r) place = r;
         continue;
       }
@@ -257,7 +287,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
       for (int i = 0; i < VPT; ++i)
         if (lane == src && i == bi) {
           xv = x[i];
-          key[i] = 0u;
+          key[i] = RX_NONE;
         }
       const int e = __shfl_sync(0xffffffffu, first + bi, src);
       xv = __shfl_sync(0xffffffffu, xv, src);
@@ -269,7 +299,8 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     }
   }
 
-  float s = my_idx >= 0 ? score(my_x) : 0.0f;
+  float s = 0.0f;
+  if (my_idx >= 0) s = p.softmax ? expf(my_x - mx) * inv : __fdividef(1.0f, 1.0f + expf(-my_x));
   if (p.renormalize) {
     const float total = warp_sum(s) + 1e-20f;
     s = __fdiv_rn(s, total);
@@ -302,15 +333,11 @@ struct RouteExpertsBwdArgs {
  */
 template <typename T, int VPT>
 __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_backward_kernel(const __grid_constant__ RouteExpertsBwdArgs p) {
-  extern __shared__ float rx_ds[];                        // per warp: 32 * VPT values of ds
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long t = static_cast<long long>(blockIdx.x) * RX_WARPS + warp;
   if (t >= p.T) return;
   const int first = lane * VPT;
   const T* row = static_cast<const T*>(p.logits) + t * p.row_stride;
-  float* ds = rx_ds + warp * 32 * VPT;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) ds[i * 32 + lane] = 0.0f;
 
   int e = -1;
   float g = 0.0f, l = 0.0f;
@@ -347,16 +374,10 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_backward_kernel(c
     d = __fdiv_rn(g - __fdiv_rn(gs, D), D);
     dot = __fdiv_rn(gs, D) * __fdiv_rn(1e-20f, D);
   }
-  __syncwarp();
-  if (e >= 0) atomicAdd(ds + e, p.softmax ? d : d * (ex * r1 * r1));
-  __syncwarp();
-
+  // Every expert's value without a pick, then the picks over them.
   float o[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const float v = ds[first + i];
-    o[i] = p.softmax ? x[i] * inv * (v - dot) : v;
-  }
+  for (int i = 0; i < VPT; ++i) o[i] = p.softmax ? -(x[i] * inv) * dot : 0.0f;
   T* out = static_cast<T*>(p.grad_logits) + t * p.E;
   if (p.E == 32 * VPT && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
     constexpr int BYTES = VPT * static_cast<int>(sizeof(T)) < 16 ? VPT * static_cast<int>(sizeof(T)) : 16;
@@ -380,6 +401,8 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_backward_kernel(c
     for (int i = 0; i < VPT; ++i)
       if (first + i < p.E) out[first + i] = from_f32<T>(o[i]);
   }
+  __syncwarp();                                           // orders the two stores of a picked expert
+  if (e >= 0) out[e] = from_f32<T>(p.softmax ? s * (d - dot) : d * (ex * r1 * r1));
 }
 
 // Experts per lane of the smallest instance that holds E experts.
@@ -392,7 +415,10 @@ inline int rx_vpt(int E) {
 template <typename T>
 inline void launch_route_experts_t(const RouteExpertsArgs& p, cudaStream_t st) {
   const unsigned grid = (static_cast<unsigned>(p.T) + RX_WARPS - 1) / RX_WARPS;
-  const size_t smem = p.n_group > 1 ? sizeof(float) * RX_WARPS * static_cast<size_t>(p.E + p.n_group) : 0;
+  // Shared keys only for groups that are not made of whole lanes.
+  const int vpt = rx_vpt(p.E), lanes = p.E / p.n_group / vpt;
+  const bool whole = p.E == 32 * vpt && lanes >= 1 && (lanes & (lanes - 1)) == 0;
+  const size_t smem = p.n_group > 1 && !whole ? sizeof(float) * RX_WARPS * static_cast<size_t>(p.E + p.n_group) : 0;
   switch (rx_vpt(p.E)) {
     case 1: route_experts_kernel<T, 1><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
     case 2: route_experts_kernel<T, 2><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
@@ -406,15 +432,13 @@ inline void launch_route_experts_t(const RouteExpertsArgs& p, cudaStream_t st) {
 template <typename T>
 inline void launch_route_experts_backward_t(const RouteExpertsBwdArgs& p, cudaStream_t st) {
   const unsigned grid = (static_cast<unsigned>(p.T) + RX_WARPS - 1) / RX_WARPS;
-  const int vpt = rx_vpt(p.E);
-  const size_t smem = sizeof(float) * RX_WARPS * 32 * static_cast<size_t>(vpt);
-  switch (vpt) {
-    case 1: route_experts_backward_kernel<T, 1><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
-    case 2: route_experts_backward_kernel<T, 2><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
-    case 4: route_experts_backward_kernel<T, 4><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
-    case 8: route_experts_backward_kernel<T, 8><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
-    case 16: route_experts_backward_kernel<T, 16><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
-    default: route_experts_backward_kernel<T, 32><<<grid, 32 * RX_WARPS, smem, st>>>(p); break;
+  switch (rx_vpt(p.E)) {
+    case 1: route_experts_backward_kernel<T, 1><<<grid, 32 * RX_WARPS, 0, st>>>(p); break;
+    case 2: route_experts_backward_kernel<T, 2><<<grid, 32 * RX_WARPS, 0, st>>>(p); break;
+    case 4: route_experts_backward_kernel<T, 4><<<grid, 32 * RX_WARPS, 0, st>>>(p); break;
+    case 8: route_experts_backward_kernel<T, 8><<<grid, 32 * RX_WARPS, 0, st>>>(p); break;
+    case 16: route_experts_backward_kernel<T, 16><<<grid, 32 * RX_WARPS, 0, st>>>(p); break;
+    default: route_experts_backward_kernel<T, 32><<<grid, 32 * RX_WARPS, 0, st>>>(p); break;
   }
 }
 
