@@ -97,9 +97,18 @@ __device__ __forceinline__ void load_row(const T* row, int first, int E, bool ve
   }
 }
 
-// Scores for the choice: e^x by the hardware's 2^x (relative error below 2^-21 for logits of any size that matter). The
+// Scores for the choice: the hardware's 2^x and 1/x (relative errors below 2^-21 for logits of any size that matter). The
 // weights use expf.
-__device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float exp_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + exp_fast(-x)));
+  return y;
+}
 
 // Key of a pick: larger pick, larger key. x + 0 makes -0 and +0 equal and every NaN the positive one, the largest key:
 // a NaN is chosen and its weight shows it.
@@ -136,7 +145,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     mx = warp_max(mx);
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) sum += __expf(x[i] - mx);
+    for (int i = 0; i < VPT; ++i) sum += exp_fast(x[i] - mx);
     inv = 1.0f / warp_sum(sum);
   }
   const bool grouped = p.n_group > 1;
@@ -156,7 +165,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const float v = __fadd_rn(p.softmax ? __expf(x[i] - mx) * inv : sigmoid_fast(x[i]), b[i]);
+      const float v = __fadd_rn(p.softmax ? exp_fast(x[i] - mx) * inv : sigmoid_fast(x[i]), b[i]);
       key[i] = x[i] == -INFINITY ? RX_NONE : pick_key(v);
     }
   }
@@ -177,11 +186,14 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
         k1 = max(k1, o1);
       }
       const uint32_t mine = p.group_top2 ? pick_key(__fadd_rn(key_value(k1), key_value(k2))) : k1;
+      // The group's lanes share the comparisons with the other groups.
       int rank = 0;
-      for (int o = 0; o < p.n_group; ++o) {
-        const uint32_t other = __shfl_sync(0xffffffffu, mine, o * lanes);
-        rank += (other > mine || (other == mine && o * lanes < (lane & ~(lanes - 1)))) ? 1 : 0;
+      const int own = lane & ~(lanes - 1);
+      for (int o = (lane - own) * lanes; o < 32 + (lane - own) * lanes; o += lanes * lanes) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, o & 31);
+        rank += o < 32 && (other > mine || (other == mine && o < own)) ? 1 : 0;
       }
+      for (int o = 1; o < lanes; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
       if (rank >= p.topk_group) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) key[i] = RX_NONE;
@@ -302,8 +314,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
   float s = 0.0f;
   if (my_idx >= 0) s = p.softmax ? expf(my_x - mx) * inv : __fdividef(1.0f, 1.0f + expf(-my_x));
   if (p.renormalize) {
-    const float total = warp_sum(s) + 1e-20f;
-    s = __fdiv_rn(s, total);
+    s = __fdividef(s, warp_sum(s) + 1e-20f);
   }
   if (place < p.k) {
     p.idx[t * p.k + place] = my_idx;
