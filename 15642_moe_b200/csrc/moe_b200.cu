@@ -683,6 +683,7 @@ bool w4_rows_aligned(const void* codes, int K) { return w4_bytes(K) % 16 == 0 &&
 // Tokens per tile: the accumulators are as small as the largest expected tile allows, so that more of them fit.
 int wm_tile(long long rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
+constexpr int WM_MAX_ROWS = 65535;   // rows of x: a grid dimension of the kernels around the products
 constexpr int WM_SMS = 148;   // the split rule's SM count: results and workspace sizes do not depend on the device
 
 // linear_w4: parts of the columns, so that few row tiles still fill the SMs; two steps each at least.
@@ -978,6 +979,7 @@ int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* code
                   int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be bf16 or f16");
   if (M < 0 || N < 1 || K < 1) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be [M, K] and W [N, K]");
+  if (M > WM_MAX_ROWS) return fail(MOE_ERR_INVALID, "moe_linear_w4: M must be at most 65535");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_linear_w4: group must be 32, 64 or 128");
   if (M == 0) return MOE_OK;
   if (!x || !codes || !scale || !out) return fail(MOE_ERR_INVALID, "moe_linear_w4: null pointer argument");
@@ -997,7 +999,7 @@ int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* code
 }
 
 size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I) {
-  if (T < 0 || T > MAX_TOKENS || top_k < 1 || top_k > RX_MAX_K || E < 1 || E > RX_MAX_E || H < 1 || I < 1) return 0;
+  if (T < 0 || T > WM_MAX_ROWS || top_k < 1 || top_k > RX_MAX_K || E < 1 || E > RX_MAX_E || H < 1 || I < 1) return 0;
   return make_experts_w4_ws(T, top_k, E, H, I).total;
 }
 
@@ -1006,7 +1008,7 @@ int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx,
                    const void* w2_zero, int group, int T, int top_k, int E, int local_offset, int H, int I, void* out,
                    void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_experts_w4: x must be bf16 or f16");
-  if (T < 0 || T > MAX_TOKENS) return fail(MOE_ERR_INVALID, "moe_experts_w4: T must be 0 to 65536");
+  if (T < 0 || T > WM_MAX_ROWS) return fail(MOE_ERR_INVALID, "moe_experts_w4: T must be 0 to 65535");
   if (top_k < 1 || top_k > RX_MAX_K) return fail(MOE_ERR_INVALID, "moe_experts_w4: top_k must be 1 to 32");
   if (E < 1 || E > RX_MAX_E) return fail(MOE_ERR_INVALID, "moe_experts_w4: E must be 1 to 1024");
   if (H < 1 || I < 1) return fail(MOE_ERR_INVALID, "moe_experts_w4: H and I must be at least 1");

@@ -12,39 +12,61 @@ several experts are stacked in a leading dimension.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native
-from .layer import _check
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SCORE = {"sigmoid": 0, "softmax": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
-MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS, MAX_TOKENS = 1024, 32, 32, 65536
+MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS, MAX_ROWS = 1024, 32, 32, 65535
 W4_GROUPS = (32, 64, 128)
 
 
-def _call(fn, device: torch.device, *args) -> None:
-    """One C call on `device` and its current stream."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, stream)
+# The handle of a device's current stream. torch.cuda.current_stream() builds a Stream object around it, which takes
+# longer than the smallest kernels here.
+_current_stream = torch._C._cuda_getCurrentRawStream
+_lib = None
+
+
+def _native_lib():
+    global _lib
+    if _lib is None:
+        _lib = _native.cuda_lib()
+    return _lib
+
+
+def _call(fn, index: int, *args) -> None:
+    """One C call on device `index` and its current stream."""
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _current_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _current_stream(index))
     if rc:
         _native.check(rc)
 
 
+def _fail(message: str) -> None:
+    raise RuntimeError(message)
+
+
 # ------------------------------------------------------------------------------------ router
-def _logits(logits) -> tuple[int, int]:
-    _check(logits.dim() == 2, "logits must be [T, E]")
-    _check(logits.dtype in _DTYPE, "logits must be float32, bfloat16 or float16")
-    _check(logits.is_cuda, "logits must be a CUDA tensor")
+# The messages are built only where a check fails: a call is a few microseconds in all.
+def _check_logits(logits) -> None:
+    if logits.dim() != 2:
+        _fail("logits must be [T, E]")
+    if logits.dtype not in _DTYPE:
+        _fail("logits must be float32, bfloat16 or float16")
+    if not logits.is_cuda:
+        _fail("logits must be a CUDA tensor")
     T, E = logits.shape
-    _check(1 <= E <= MAX_EXPERTS, f"logits must have 1 to {MAX_EXPERTS} experts")
-    _check(T == 0 or logits.stride(1) == 1 or E == 1, "logits must have neighbouring experts in memory (stride 1)")
-    return T, E
+    if not 1 <= E <= MAX_EXPERTS:
+        _fail(f"logits must have 1 to {MAX_EXPERTS} experts")
+    if E > 1 and T > 0 and logits.stride(1) != 1:
+        _fail("logits must have neighbouring experts in memory (stride 1)")
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: torch.Tensor | None = None,
@@ -66,24 +88,32 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     """
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteExperts.apply(logits, top_k, score, bias, n_group, topk_group, group_score, renormalize, scale)
-    T, E = _logits(logits)
-    _check(score in _SCORE, "score must be 'softmax' or 'sigmoid'")
-    _check(group_score in _GROUP_SCORE, "group_score must be 'max' or 'top2'")
-    _check(1 <= n_group <= MAX_GROUPS and E % n_group == 0, f"n_group must divide the experts and be 1 to {MAX_GROUPS}")
-    _check(1 <= topk_group <= n_group, "topk_group must be 1 to n_group")
-    _check(1 <= top_k <= min(MAX_TOP_K, E // n_group * topk_group),
-           f"top_k must be 1 to {MAX_TOP_K} and at most the experts of topk_group groups")
-    _check(n_group == 1 or group_score == "max" or E // n_group >= 2, "group_score 'top2' needs two experts per group")
+    _check_logits(logits)
+    T, E = logits.shape
+    if score not in _SCORE:
+        _fail("score must be 'softmax' or 'sigmoid'")
+    if group_score not in _GROUP_SCORE:
+        _fail("group_score must be 'max' or 'top2'")
+    if not (1 <= n_group <= MAX_GROUPS and E % n_group == 0):
+        _fail(f"n_group must divide the experts and be 1 to {MAX_GROUPS}")
+    if not 1 <= topk_group <= n_group:
+        _fail("topk_group must be 1 to n_group")
+    if not 1 <= top_k <= min(MAX_TOP_K, E // n_group * topk_group):
+        _fail(f"top_k must be 1 to {MAX_TOP_K} and at most the experts of topk_group groups")
+    if n_group > 1 and group_score == "top2" and E // n_group < 2:
+        _fail("group_score 'top2' needs two experts per group")
+    index, bias_ptr = logits.get_device(), None
     if bias is not None:
-        _check(bias.dtype == torch.float32 and bias.dim() == 1 and bias.shape[0] == E and bias.is_contiguous()
-               and bias.device == logits.device, "bias must be a contiguous float32 [E] tensor on the logits' device")
-    dev = logits.device
-    idx = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+        if not (bias.dtype == torch.float32 and bias.dim() == 1 and bias.shape[0] == E and bias.is_contiguous()
+                and bias.is_cuda and bias.get_device() == index):
+            _fail("bias must be a contiguous float32 [E] tensor on the logits' device")
+        bias_ptr = bias.data_ptr()
+    w = logits.new_empty((T, top_k), dtype=torch.float32)
+    idx = torch.empty_like(w, dtype=torch.int32)
     if T:
-        _call(_native.cuda_lib().moe_route_experts, dev, logits.data_ptr(), _DTYPE[logits.dtype], logits.stride(0),
-              None if bias is None else bias.data_ptr(), T, E, top_k, _SCORE[score], n_group, topk_group,
-              _GROUP_SCORE[group_score], 1 if renormalize else 0, scale, idx.data_ptr(), w.data_ptr())
+        _call(_native_lib().moe_route_experts, index, logits.data_ptr(), _DTYPE[logits.dtype], logits.stride(0),
+              bias_ptr, T, E, top_k, _SCORE[score], n_group, topk_group, _GROUP_SCORE[group_score],
+              1 if renormalize else 0, scale, idx.data_ptr(), w.data_ptr())
     return idx, w
 
 
@@ -94,18 +124,20 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, idx
     ``grad_weights`` fp32 [T, top_k], ``idx`` int32 [T, top_k] as route_experts returned it (distinct experts per
     row; -1 takes no part), and the forward call's ``score``, ``renormalize`` and ``scale``. The choice of the
     experts has no gradient."""
-    T, E = _logits(logits)
-    _check(score in _SCORE, "score must be 'softmax' or 'sigmoid'")
-    _check(idx.dim() == 2 and idx.shape[0] == T and 1 <= idx.shape[1] <= MAX_TOP_K and idx.dtype == torch.int32
-           and idx.is_contiguous() and idx.device == logits.device,
-           f"idx must be a contiguous int32 [T, top_k] tensor on the logits' device, top_k 1 to {MAX_TOP_K}")
-    _check(grad_weights.shape == idx.shape and grad_weights.dtype == torch.float32 and grad_weights.is_contiguous()
-           and grad_weights.device == logits.device,
-           "grad_weights must be a contiguous float32 [T, top_k] tensor on the logits' device")
-    dev = logits.device
-    grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    _check_logits(logits)
+    T, E = logits.shape
+    if score not in _SCORE:
+        _fail("score must be 'softmax' or 'sigmoid'")
+    index = logits.get_device()
+    if not (idx.dim() == 2 and idx.shape[0] == T and 1 <= idx.shape[1] <= MAX_TOP_K and idx.dtype == torch.int32
+            and idx.is_contiguous() and idx.is_cuda and idx.get_device() == index):
+        _fail(f"idx must be a contiguous int32 [T, top_k] tensor on the logits' device, top_k 1 to {MAX_TOP_K}")
+    if not (grad_weights.shape == idx.shape and grad_weights.dtype == torch.float32 and grad_weights.is_contiguous()
+            and grad_weights.is_cuda and grad_weights.get_device() == index):
+        _fail("grad_weights must be a contiguous float32 [T, top_k] tensor on the logits' device")
+    grad = logits.new_empty((T, E))
     if T:
-        _call(_native.cuda_lib().moe_route_experts_backward, dev, grad_weights.data_ptr(), logits.data_ptr(),
+        _call(_native_lib().moe_route_experts_backward, index, grad_weights.data_ptr(), logits.data_ptr(),
               _DTYPE[logits.dtype], logits.stride(0), idx.data_ptr(), T, E, idx.shape[1], _SCORE[score],
               1 if renormalize else 0, scale, grad.data_ptr())
     return grad
@@ -129,52 +161,70 @@ class _RouteExperts(torch.autograd.Function):
 
 
 # ----------------------------------------------------------------------------- 4-bit products
-def _w4(codes, scale, zero, group, lead, N, K, dtype, dev, name) -> None:
-    """Checks one 4-bit matrix (or a stack of them) of N rows and K columns."""
-    _check(codes.dtype == torch.uint8 and codes.shape == (*lead, N, (K + 1) // 2) and codes.is_contiguous(),
-           f"{name} must be a contiguous uint8 tensor of shape {[*lead, N, (K + 1) // 2]}")
-    shape = (*lead, N, -(-K // group))
-    _check(scale.dtype == dtype and scale.shape == shape and scale.is_contiguous(),
-           f"{name}'s scale must be a contiguous {dtype} tensor of shape {list(shape)}")
-    _check(codes.device == dev and scale.device == dev, "all tensors must be on one device")
-    if zero is not None:
-        _check(zero.dtype == torch.uint8 and zero.shape == shape and zero.is_contiguous() and zero.device == dev,
-               f"{name}'s zero must be a contiguous uint8 tensor of shape {list(shape)} on the same device")
+def _w4(codes, scale, zero, group, shape, K, dtype, index, name) -> None:
+    """Checks one 4-bit matrix (or a stack of them): `shape` without the columns, K columns."""
+    if not (codes.dtype == torch.uint8 and codes.shape == (*shape, (K + 1) // 2) and codes.is_contiguous()):
+        _fail(f"{name} must be a contiguous uint8 tensor of shape {[*shape, (K + 1) // 2]}")
+    groups = (*shape, -(-K // group))
+    if not (scale.dtype == dtype and scale.shape == groups and scale.is_contiguous()):
+        _fail(f"{name}'s scale must be a contiguous {dtype} tensor of shape {list(groups)}")
+    if not (codes.is_cuda and codes.get_device() == index and scale.is_cuda and scale.get_device() == index):
+        _fail("all tensors must be on one device")
+    if zero is not None and not (zero.dtype == torch.uint8 and zero.shape == groups and zero.is_contiguous()
+                                 and zero.is_cuda and zero.get_device() == index):
+        _fail(f"{name}'s zero must be a contiguous uint8 tensor of shape {list(groups)} on the same device")
+
+
+def _check_x(x, group, what) -> None:
+    if x.dim() != 2:
+        _fail(f"x must be {what}")
+    if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
+        _fail("x must be bfloat16 or float16")
+    if not x.is_cuda:
+        _fail("x must be a CUDA tensor")
+    if group not in W4_GROUPS:
+        _fail("group must be 32, 64 or 128")
+    if x.shape[0] > 0 and x.shape[1] > 1 and x.stride(1) != 1:
+        _fail("x must have neighbouring columns in memory (stride 1)")
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_w4_workspace_bytes(M: int, N: int, K: int) -> int:
+    return int(_native_lib().moe_linear_w4_workspace_bytes(M, N, K))
 
 
 def linear_w4(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None, *,
               group: int = 128, out: torch.Tensor | None = None) -> torch.Tensor:
     """x [M, K] (bfloat16 or float16, rows any distance apart) times the 4-bit W [N, K]: [M, N] in x's type.
 
-    ``codes``, ``scale``, ``zero`` as in this module's description, ``group`` 32, 64 or 128. Any M, N and K from 1
-    on. Sums are held in 32 bits and rounded once."""
-    _check(x.dim() == 2, "x must be [M, K]")
-    _check(x.dtype == torch.bfloat16 or x.dtype == torch.float16, "x must be bfloat16 or float16")
-    _check(x.is_cuda, "x must be a CUDA tensor")
-    _check(group in W4_GROUPS, "group must be 32, 64 or 128")
-    _check(codes.dim() == 2, "codes must be [N, ceil(K / 2)]")
-    (M, K), N, dev = x.shape, codes.shape[0], x.device
-    _check(K >= 1 and N >= 1, "x and codes must have at least one column and one row")
-    _check(M == 0 or K == 1 or x.stride(1) == 1, "x must have neighbouring columns in memory (stride 1)")
-    _w4(codes, scale, zero, group, (), N, K, x.dtype, dev, "codes")
+    ``codes``, ``scale``, ``zero`` as in this module's description, ``group`` 32, 64 or 128. M up to 65535, any N and
+    K from 1 on. Sums are held in 32 bits and rounded once."""
+    _check_x(x, group, "[M, K]")
+    if codes.dim() != 2:
+        _fail("codes must be [N, ceil(K / 2)]")
+    (M, K), N, index = x.shape, codes.shape[0], x.get_device()
+    if not (K >= 1 and N >= 1):
+        _fail("x and codes must have at least one column and one row")
+    if M > MAX_ROWS:
+        _fail(f"x must have at most {MAX_ROWS} rows")
+    _w4(codes, scale, zero, group, (N,), K, x.dtype, index, "codes")
     if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=dev)
-    else:
-        _check(out.dtype == x.dtype and out.shape == (M, N) and out.is_contiguous() and out.device == dev,
-               "out must be a contiguous [M, N] tensor of x's type on its device")
+        out = x.new_empty((M, N))
+    elif not (out.dtype == x.dtype and out.shape == (M, N) and out.is_contiguous() and out.is_cuda
+              and out.get_device() == index):
+        _fail("out must be a contiguous [M, N] tensor of x's type on its device")
     if M:
-        lib, ws, need = _native.cuda_lib(), None, 0
-        if M > 8:
-            need = int(lib.moe_linear_w4_workspace_bytes(M, N, K))
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call(lib.moe_linear_w4, dev, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), codes.data_ptr(), scale.data_ptr(),
-              None if zero is None else zero.data_ptr(), group, M, N, K, out.data_ptr(),
-              None if ws is None else ws.data_ptr(), need)
+        need = _linear_w4_workspace_bytes(M, N, K)
+        ws = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
+        _call(_native_lib().moe_linear_w4, index, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), codes.data_ptr(),
+              scale.data_ptr(), None if zero is None else zero.data_ptr(), group, M, N, K, out.data_ptr(), ws, need)
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def experts_w4_workspace_bytes(T: int, top_k: int, E: int, H: int, I: int) -> int:
-    return int(_native.cuda_lib().moe_experts_w4_workspace_bytes(T, top_k, E, H, I))
+    """Bytes of experts_w4's workspace."""
+    return int(_native_lib().moe_experts_w4_workspace_bytes(T, top_k, E, H, I))
 
 
 def experts_w4(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor,
@@ -188,41 +238,42 @@ def experts_w4(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w13: t
     halves, reference/moe_ref.py:129-130). Other picks (-1, experts of other GPUs) add nothing.
 
     ``x`` [T, H] bfloat16 or float16, rows any distance apart; ``idx`` int32 and ``weights`` fp32 [T, top_k], as
-    route_experts returns them; ``w13`` codes uint8 [E, 2 I, ceil(H / 2)], ``w2`` codes uint8 [E, H, ceil(I / 2)],
-    scales and zero points as in this module's description. Sums are held in 32 bits and rounded once."""
-    _check(x.dim() == 2, "x must be [T, H]")
-    _check(x.dtype == torch.bfloat16 or x.dtype == torch.float16, "x must be bfloat16 or float16")
-    _check(x.is_cuda, "x must be a CUDA tensor")
-    _check(group in W4_GROUPS, "group must be 32, 64 or 128")
-    _check(w13.dim() == 3 and w13.shape[1] % 2 == 0, "w13 must be [E, 2 I, ceil(H / 2)]")
-    (T, H), dev = x.shape, x.device
+    route_experts returns them; ``w13`` codes uint8 [E, 2 I, ceil(H / 2)], ``w2`` codes uint8 [E, H, ceil(I / 2)]
+    (16-byte aligned), scales and zero points as in this module's description. T up to 65535. Sums are held in 32 bits
+    and rounded once."""
+    _check_x(x, group, "[T, H]")
+    if not (w13.dim() == 3 and w13.shape[1] % 2 == 0):
+        _fail("w13 must be [E, 2 I, ceil(H / 2)]")
+    (T, H), index = x.shape, x.get_device()
     E, I = w13.shape[0], w13.shape[1] // 2
-    _check(1 <= E <= MAX_EXPERTS and H >= 1 and I >= 1, f"w13 must hold 1 to {MAX_EXPERTS} experts")
-    _check(T <= MAX_TOKENS, f"x must have at most {MAX_TOKENS} tokens")
-    _check(T == 0 or H == 1 or x.stride(1) == 1, "x must have neighbouring columns in memory (stride 1)")
-    _check(idx.dim() == 2 and idx.shape[0] == T and 1 <= idx.shape[1] <= MAX_TOP_K and idx.dtype == torch.int32
-           and idx.is_contiguous() and idx.device == dev,
-           f"idx must be a contiguous int32 [T, top_k] tensor on x's device, top_k 1 to {MAX_TOP_K}")
-    _check(weights.shape == idx.shape and weights.dtype == torch.float32 and weights.is_contiguous()
-           and weights.device == dev, "weights must be a contiguous float32 [T, top_k] tensor on x's device")
-    _w4(w13, w13_scale, w13_zero, group, (E,), 2 * I, H, x.dtype, dev, "w13")
-    _w4(w2, w2_scale, w2_zero, group, (E,), H, I, x.dtype, dev, "w2")
+    if not (1 <= E <= MAX_EXPERTS and H >= 1 and I >= 1):
+        _fail(f"w13 must hold 1 to {MAX_EXPERTS} experts")
+    if T > MAX_ROWS:
+        _fail(f"x must have at most {MAX_ROWS} tokens")
+    if not (idx.dim() == 2 and idx.shape[0] == T and 1 <= idx.shape[1] <= MAX_TOP_K and idx.dtype == torch.int32
+            and idx.is_contiguous() and idx.is_cuda and idx.get_device() == index):
+        _fail(f"idx must be a contiguous int32 [T, top_k] tensor on x's device, top_k 1 to {MAX_TOP_K}")
+    if not (weights.shape == idx.shape and weights.dtype == torch.float32 and weights.is_contiguous()
+            and weights.is_cuda and weights.get_device() == index):
+        _fail("weights must be a contiguous float32 [T, top_k] tensor on x's device")
+    _w4(w13, w13_scale, w13_zero, group, (E, 2 * I), H, x.dtype, index, "w13")
+    _w4(w2, w2_scale, w2_zero, group, (E, H), I, x.dtype, index, "w2")
     if out is None:
-        out = torch.empty((T, H), dtype=x.dtype, device=dev)
-    else:
-        _check(out.dtype == x.dtype and out.shape == (T, H) and out.is_contiguous() and out.device == dev,
-               "out must be a contiguous [T, H] tensor of x's type on its device")
+        out = x.new_empty((T, H))
+    elif not (out.dtype == x.dtype and out.shape == (T, H) and out.is_contiguous() and out.is_cuda
+              and out.get_device() == index):
+        _fail("out must be a contiguous [T, H] tensor of x's type on its device")
     if T == 0:
         return out
-    lib, top_k = _native.cuda_lib(), idx.shape[1]
-    need = int(lib.moe_experts_w4_workspace_bytes(T, top_k, E, H, I))
+    top_k = idx.shape[1]
+    need = experts_w4_workspace_bytes(T, top_k, E, H, I)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    else:
-        _check(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev
-               and workspace.numel() >= need, f"workspace must be a contiguous uint8 tensor of at least {need} bytes on x's device")
-    _call(lib.moe_experts_w4, dev, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), idx.data_ptr(), weights.data_ptr(),
-          w13.data_ptr(), w13_scale.data_ptr(), None if w13_zero is None else w13_zero.data_ptr(), w2.data_ptr(),
-          w2_scale.data_ptr(), None if w2_zero is None else w2_zero.data_ptr(), group, T, top_k, E, local_offset, H, I,
-          out.data_ptr(), workspace.data_ptr(), workspace.numel())
+        workspace = x.new_empty(need, dtype=torch.uint8)
+    elif not (workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need
+              and workspace.is_cuda and workspace.get_device() == index):
+        _fail(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on x's device")
+    _call(_native_lib().moe_experts_w4, index, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), idx.data_ptr(),
+          weights.data_ptr(), w13.data_ptr(), w13_scale.data_ptr(), None if w13_zero is None else w13_zero.data_ptr(),
+          w2.data_ptr(), w2_scale.data_ptr(), None if w2_zero is None else w2_zero.data_ptr(), group, T, top_k, E,
+          local_offset, H, I, out.data_ptr(), workspace.data_ptr(), workspace.numel())
     return out

@@ -42,7 +42,7 @@ def test_products_refuse(lib, ptr):
     p = ptr[0]
     call = lambda dtype=1, group=128, M=2, N=8, K=64, x=p: lib.moe_linear_w4(  # noqa: E731
         x, dtype, 64, p, p, None, group, M, N, K, p, None, 0, None)
-    for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=16), b"group"), (dict(M=-1), b"[M, K]"), (dict(N=0), b"[M, K]"),
+    for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=16), b"group"), (dict(M=-1), b"[M, K]"), (dict(M=65536), b"65535"), (dict(N=0), b"[M, K]"),
                      (dict(K=0), b"[M, K]"), (dict(x=None), b"null")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
     assert call(M=0) == 0
@@ -50,14 +50,14 @@ def test_products_refuse(lib, ptr):
     assert lib.moe_linear_w4_workspace_bytes(8, 64, 64) == 0 and lib.moe_linear_w4_workspace_bytes(9, 64, 64) > 0
     call = lambda dtype=1, group=128, T=2, k=2, E=4, H=64, I=32, ws=p, n=0, x=p: lib.moe_experts_w4(  # noqa: E731
         x, dtype, 64, p, p, p, p, None, p, p, None, group, T, k, E, 0, H, I, p, ws, n, None)
-    for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=1), b"group"), (dict(T=65537), b"65536"), (dict(k=0), b"top_k"),
+    for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=1), b"group"), (dict(T=65536), b"65535"), (dict(k=0), b"top_k"),
                      (dict(E=1025), b"E must"), (dict(H=0), b"H and I"), (dict(x=None), b"null"), (dict(ws=None), b"null")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
     assert call(n=16) == 3 and b"workspace too small" in lib.moe_last_error()
     assert call(T=0) == 0
     need = lib.moe_experts_w4_workspace_bytes(2, 2, 4, 64, 32)
-    assert need > 0 and lib.moe_experts_w4_workspace_bytes(65536, 32, 256, 7168, 2048) > need
-    assert lib.moe_experts_w4_workspace_bytes(65537, 2, 4, 64, 32) == 0
+    assert need > 0 and lib.moe_experts_w4_workspace_bytes(65535, 32, 256, 7168, 2048) > need
+    assert lib.moe_experts_w4_workspace_bytes(65536, 2, 4, 64, 32) == 0
     assert call(ws=p + 16, n=1 << 40) == 1 and b"256-byte aligned" in lib.moe_last_error()
 
 
