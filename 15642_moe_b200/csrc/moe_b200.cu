@@ -842,15 +842,8 @@ template <typename T>
 int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Matrix& w, int M, int N, int K, void* out, void* workspace,
                    cudaStream_t st) {
   if (M <= WS_TOK) {
-    const int steps = (K + WS_STEP - 1) / WS_STEP, tiles = (N + WS_ROWS - 1) / WS_ROWS;
-    // Split the columns over a cluster until there are two blocks per SM, with two steps each at least.
-    int cluster = 1;
-    while (cluster < 8 && tiles * cluster < 2 * d->num_sms && steps >= 4 * cluster) cluster *= 2;
-    StreamArgs a{x, x_stride, w, M, N, K, 1, 0, 0, nullptr, nullptr, 0, 1, 0, nullptr, out};
-    a.parts = cluster > (steps + WS_CHUNK - 1) / WS_CHUNK ? cluster : (steps + WS_CHUNK - 1) / WS_CHUNK;
-    a.spp = (steps + a.parts - 1) / a.parts;
-    a.parts = (steps + a.spp - 1) / a.spp;
-    return cuda_check(launch_w4_stream<T, WS_LINEAR>(a, cluster, 1, false, st), "linear_w4 launch");
+    const StreamArgs a{x, x_stride, w, M, N, K, out};
+    return cuda_check(launch_w4_stream<T>(a, st), "linear_w4 launch");
   }
   const LinearW4Ws ws = make_linear_w4_ws(M, N, K);
   uint8_t* W = static_cast<uint8_t*>(workspace);

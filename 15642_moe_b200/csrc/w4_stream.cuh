@@ -1,20 +1,18 @@
 /*
- * Products with 4-bit weights for up to 8 tokens: the weights are read once, straight from global memory
- * into matrix fragments, and that read is all the time there is (6.45 TB/s measured).
+ * linear_w4 for up to 8 tokens, in one launch: the weights are read once, straight from global memory into matrix
+ * fragments.
  *
  *   mma m16n8k16: A = 16 weight rows x 16 columns, B = 16 columns x 8 tokens, fp32 accumulators.
  *
- * A thread holds, of rows g and g + 8 of a tile, the four codes at each of two places; which columns those
- * are is free as long as A and B agree. So thread t of a row's four takes g/4 neighbouring columns of each
- * group of g (one 16-, 8- or 4-byte load), a 32-bit word of 8 codes makes the fragments of two mma, and the
- * activations are put into shared memory in that order once per block. Codes become numbers by placing a
- * nibble in the mantissa of 128 (bf16) or 1024 (f16) and subtracting 128 + zero: exact, as is every product.
- * Each group's sum is scaled in fp32: no weight is ever rounded.
+ * A thread holds, of rows g and g + 8 of a tile, the codes at a few places; which columns those are is free as long as A
+ * and B agree. Thread t of a row's four takes group / 4 neighbouring columns of each group (one 16-, 8- or 4-byte load); a
+ * 32-bit word of 8 codes makes the fragments of two mma. Codes become numbers by placing a nibble in the mantissa of 128
+ * (bf16) or 1024 (f16) and subtracting 128 + zero or 1024 + zero: exact, as is every product. Each group's sum is scaled in
+ * fp32: no weight is rounded.
  *
- * Split: a block has 8 warps, 4 tiles of 16 rows x 2 column halves; a cluster of up to 8 blocks shares the
- * same rows and splits the columns (for the experts' second product: the active experts and their columns),
- * and adds its parts through distributed shared memory in rank order, so results repeat bit for bit.
- * Each warp keeps 4 steps of 128 columns in flight (4 KB).
+ * Split: a block has one tile of 16 rows, its 8 warps an eighth of the columns each; their sums meet in shared memory in
+ * warp order, so results repeat bit for bit. Nothing is staged: a warp alone uses its columns of x. 4 steps of 128 columns
+ * are in flight per warp (4 KB).
  */
 #pragma once
 #include "gate.cuh"
@@ -25,28 +23,19 @@
 namespace moe {
 
 constexpr int WS_WARPS = 8, WS_THREADS = 32 * WS_WARPS;
-constexpr int WS_WK = 2;                        // column halves per block
-constexpr int WS_ROWS = 16 * WS_WARPS / WS_WK;  // 64 weight rows per block
+constexpr int WS_ROWS = 16;                     // weight rows per block
 constexpr int WS_TOK = 8;                       // tokens per mma
 constexpr int WS_STEP = 128;                    // columns per step
-constexpr int WS_CHUNK = 16;                    // steps staged at a time
 constexpr int WS_DEPTH = 4;                     // steps in flight per warp
-constexpr int WS_MAX_PICKS = WS_TOK * RX_MAX_K; // 256
 
-enum { WS_LINEAR = 0, WS_UP = 1, WS_DOWN = 2 };
+enum { WS_LINEAR = 0, WS_UP = 1, WS_DOWN = 2 };  // which product a kernel computes: linear_w4, the experts' first, second
 
 struct StreamArgs {
-  const void* x;           // [M, K] (linear, up)
+  const void* x;           // [M, K]
   long long x_stride;
   W4Matrix w;
-  int M, N, K;             // tokens (<= 8); output columns (up: I); reduction length
-  int cluster;             // blocks per cluster: gridDim.x = row tiles * cluster
-  int parts, spp;          // the K steps of one matrix in `parts` parts of `spp` steps (down: parts at least)
-  const int* idx;          // [M, k] (up, down)
-  const float* wt;         // [M, k] (down)
-  int k, E, offset;
-  float* h;                // [M * k, M, I]: entry (r, t) is token t through the expert first picked at r
-  void* out;               // [M, N] (linear, down)
+  int M, N, K;             // tokens (<= 8), output columns, reduction length
+  void* out;               // [M, N]
 };
 
 // mma with bf16 or f16 operands: d += a x b.
@@ -155,321 +144,112 @@ __device__ __forceinline__ uint4 ld_x_pairs(const T* row, int k, int K, bool vec
   return make_uint4(pack2(e[0], e[4]), pack2(e[1], e[5]), pack2(e[2], e[6]), pack2(e[3], e[7]));
 }
 
-// The same for 8 fp32 values, as two bf16 terms (hi + lo carry 16 bits).
-__device__ __forceinline__ void ld_h_pairs(const float* row, int k, int K, uint4& hi, uint4& lo) {
-  float v[8];
-  if (k + 8 <= K && (reinterpret_cast<uintptr_t>(row + k) & 15u) == 0) {
-    const float4 a = *reinterpret_cast<const float4*>(row + k), b = *reinterpret_cast<const float4*>(row + k + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? row[k + i] : 0.0f;
-  }
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    h[i] = pack_bf16x2(v[i], v[i + 4]);
-    const float r0 = v[i] - __uint_as_float(h[i] << 16), r1 = v[i + 4] - __uint_as_float(h[i] & 0xFFFF0000u);
-    // A value past bf16's range (or NaN) has no remainder.
-    l[i] = pack_bf16x2(fabsf(r0) <= 3.4e38f ? r0 : 0.0f, fabsf(r1) <= 3.4e38f ? r1 : 0.0f);
-  }
-  hi = make_uint4(h[0], h[1], h[2], h[3]);
-  lo = make_uint4(l[0], l[1], l[2], l[3]);
-}
-
-// Shared memory of one block, in bytes: activations of a chunk, then scales and offsets of its groups.
-inline size_t ws_smem(int mode, int M, int chunk_steps, int group) {
-  return static_cast<size_t>(chunk_steps) * 16 * M * 16 * (mode == WS_DOWN ? 2 : 1) +
-         static_cast<size_t>(WS_ROWS) * (chunk_steps * (WS_STEP / group) + 1) * 8;
-}
-
-template <typename T, int G4, int MODE, bool ALIGNED>
-__global__ void __launch_bounds__(WS_THREADS, 3) w4_stream_kernel(const __grid_constant__ StreamArgs p) {
-  using W = typename std::conditional<MODE == WS_DOWN, __nv_bfloat16, T>::type;   // type of the fragments
-  constexpr int NB = MODE == WS_DOWN ? 2 : 1;
+template <typename T, int G4, bool ALIGNED>
+__global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_constant__ StreamArgs p) {
   constexpr int GPS = 4 / G4;                    // groups per step
-  extern __shared__ __align__(16) uint8_t ws_dyn[];
-  __shared__ float red[WS_WK][WS_ROWS][WS_TOK];
-  __shared__ int s_idx[MODE == WS_LINEAR ? 1 : WS_MAX_PICKS];
-  __shared__ int s_act[MODE == WS_DOWN ? WS_MAX_PICKS : 1];
-  __shared__ uint32_t s_mask[WS_WARPS];
-  __shared__ float s_wt[WS_TOK];
-  __shared__ int s_routed;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int wr = warp / WS_WK, wk = warp % WS_WK;
-  const int S = p.cluster, rank = static_cast<int>(blockIdx.x) % S;
-  const int tile = static_cast<int>(blockIdx.x) / S, slot = blockIdx.y;
+  __shared__ float red[WS_WARPS][WS_ROWS][WS_TOK];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pitch = (p.K + 1) / 2, steps = (p.K + WS_STEP - 1) / WS_STEP;
   const int groups = (p.K + p.w.group - 1) / p.w.group;
-  const int picks = p.M * p.k;
+  const int per = (steps + WS_WARPS - 1) / WS_WARPS;
+  const int a = warp * per, n = min(steps, a + per) - a;            // this warp's steps (n may be 0 or less)
+  const int n0 = blockIdx.x * WS_ROWS;
+  const long long r0 = min(n0 + g, p.N - 1), r1 = min(n0 + g + 8, p.N - 1);   // rows past N repeat the last one
+  const uint8_t *c0 = p.w.codes + r0 * pitch, *c1 = p.w.codes + r1 * pitch;
+  const T *f0 = static_cast<const T*>(p.w.scale) + r0 * groups, *f1 = static_cast<const T*>(p.w.scale) + r1 * groups;
+  const uint8_t *z0 = p.w.zero ? p.w.zero + r0 * groups : nullptr, *z1 = p.w.zero ? p.w.zero + r1 * groups : nullptr;
+  const T* xrow = static_cast<const T*>(p.x) + min(g, p.M - 1) * p.x_stride;
+  const bool vec = (reinterpret_cast<uintptr_t>(xrow) & 15u) == 0;
 
-  // Which experts: `up` has one block (cluster) per pick, those whose expert an earlier pick has end here;
-  // `down` walks the list of the picks' distinct experts.
-  int expert = 0, n_act = 1, parts = p.parts, spp = p.spp;
-  if constexpr (MODE == WS_UP) {
-    for (int r = tid; r < picks; r += WS_THREADS) s_idx[r] = p.idx[r];
-    if (tid == 0) s_routed = 0;
-    __syncthreads();
-    expert = s_idx[slot] - p.offset;
-    bool skip = expert < 0 || expert >= p.E;
-    if (tid < slot && s_idx[tid] == s_idx[slot]) skip = true;
-    if (tid < picks && s_idx[tid] == s_idx[slot]) atomicOr(&s_routed, 1 << (tid / p.k));
-    if (__syncthreads_or(skip)) {
-      allow_dependent_launch();
-      return;
-    }
-    allow_dependent_launch();
-  }
-  if constexpr (MODE == WS_DOWN) {
-    if (tid < picks) s_idx[tid] = p.idx[tid];
-    __syncthreads();
-    bool first = false;
-    if (tid < picks) {
-      const int e = s_idx[tid] - p.offset;
-      first = e >= 0 && e < p.E;
-      for (int r = 0; r < tid; ++r)
-        if (s_idx[r] == s_idx[tid]) first = false;
-    }
-    const uint32_t m = __ballot_sync(0xffffffffu, first);
-    if (lane == 0) s_mask[warp] = m;
-    __syncthreads();
-    int at = __popc(m & ((1u << lane) - 1u));
-    n_act = 0;
+  uint4 buf[WS_DEPTH][2];
 #pragma unroll
-    for (int i = 0; i < WS_WARPS; ++i) {
-      if (i < warp) at += __popc(s_mask[i]);
-      n_act += __popc(s_mask[i]);
+  for (int d = 0; d < WS_DEPTH; ++d)
+    if (d < n) {
+      buf[d][0] = ld_codes<G4, ALIGNED>(c0, a + d, t, pitch);
+      buf[d][1] = ld_codes<G4, ALIGNED>(c1, a + d, t, pitch);
     }
-    if (first) s_act[at] = tid;
-    __syncthreads();
-    // Few active experts: cut their columns so that every block of the cluster has a part.
-    if (n_act > 0 && n_act * parts < S) {
-      parts = min(steps, (S + n_act - 1) / n_act);
-      spp = (steps + parts - 1) / parts;
-      parts = (steps + spp - 1) / spp;
+  // One step ahead: activations, scales and zero points.
+  uint4 x[4];
+  float s0[GPS], s1[GPS];
+  uint32_t o0[GPS], o1[GPS];
+  auto side = [&](int step) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = step * WS_STEP + (i / G4) * (32 * G4) + t * (8 * G4) + (i % G4) * 8;
+      x[i] = g < p.M ? ld_x_pairs<T>(xrow, k, p.K, vec) : make_uint4(0, 0, 0, 0);
     }
-  }
-
-  uint8_t* xs = ws_dyn;
-  const int x_units = spp * 16 * p.M;
-  float* sc = reinterpret_cast<float*>(ws_dyn + static_cast<size_t>(p.spp) * 16 * p.M * 16 * NB);
-  const int sc_pitch = p.spp * GPS + 1;
-  uint32_t* zo = reinterpret_cast<uint32_t*>(sc + WS_ROWS * sc_pitch);
-
-  // Weight rows of this thread: g and g + 8 of the warp's tile; `up` puts column i of X1 and of X2 there.
-  const int r0 = wr * 16 + g;
-  auto matrix_row = [&](int local) -> long long {   // local row 0..63 of the block -> row of the matrix, clamped
-    if constexpr (MODE == WS_UP) {
-      const int i = min(tile * (WS_ROWS / 2) + (local >> 4) * 8 + (local & 7), p.N - 1);
-      return (local & 8) ? static_cast<long long>(p.N) + i : i;
-    } else {
-      return min(tile * WS_ROWS + local, p.N - 1);
+#pragma unroll
+    for (int i = 0; i < GPS; ++i) {
+      const int q = min(step * GPS + i, groups - 1);
+      s0[i] = to_f32(f0[q]);
+      s1[i] = to_f32(f1[q]);
+      o0[i] = w4_offset<T>(z0 ? __ldg(z0 + q) & 15 : 8);
+      o1[i] = w4_offset<T>(z1 ? __ldg(z1 + q) & 15 : 8);
     }
   };
-  const int rows_per = MODE == WS_UP ? 2 * p.N : p.N;
-  const long long mr0 = matrix_row(r0), mr1 = matrix_row(r0 + 8);
-
   float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int items = n_act * parts;
-  bool waited = false;
-  for (int item = rank; item < items; item += S) {
-    const int part = item % parts;
-    int pick = 0;
-    if constexpr (MODE == WS_DOWN) {
-      pick = s_act[item / parts];
-      expert = s_idx[pick] - p.offset;
-    }
-    const int s_begin = part * spp, s_end = min(steps, s_begin + spp);
-    const int half = (s_end - s_begin + WS_WK - 1) / WS_WK;
-    const int a = s_begin + wk * half, b = min(s_end, a + half), n = b - a;
-    const long long first_row = static_cast<long long>(expert) * rows_per;
-    const uint8_t* c0 = p.w.codes + (first_row + mr0) * pitch;
-    const uint8_t* c1 = p.w.codes + (first_row + mr1) * pitch;
-    uint4 buf[WS_DEPTH][2];
+  if (n > 0) side(a);
+  for (int s = 0; s < n; s += WS_DEPTH) {
 #pragma unroll
     for (int d = 0; d < WS_DEPTH; ++d)
-      if (d < n) {
-        buf[d][0] = ld_codes<G4, ALIGNED>(c0, a + d, t, pitch);
-        buf[d][1] = ld_codes<G4, ALIGNED>(c1, a + d, t, pitch);
-      }
-    __syncthreads();                              // the last item's shared memory is free
-    // Scales and offsets of the block's rows.
-    const int g_begin = s_begin * GPS, g_count = min(groups, s_end * GPS) - g_begin;
-    for (int i = tid; i < WS_ROWS * g_count; i += WS_THREADS) {
-      const int local = i / g_count, q = i % g_count;
-      const long long at = (first_row + matrix_row(local)) * groups + g_begin + q;
-      sc[local * sc_pitch + q] = to_f32(static_cast<const T*>(p.w.scale)[at]);
-      zo[local * sc_pitch + q] = w4_offset<W>(p.w.zero ? p.w.zero[at] & 15 : 8);
-    }
-    // Activations in fragment order: unit ((step, word, token), t) of 16 bytes.
-    const int units = (s_end - s_begin) * 16;
-    if constexpr (MODE == WS_DOWN) {
-      if (tid < WS_TOK) {
-        float w = 0.0f;
-        if (tid < p.M)
-          for (int j = 0; j < p.k; ++j)
-            if (s_idx[tid * p.k + j] == s_idx[pick]) w += p.wt[tid * p.k + j];
-        s_wt[tid] = w;
-      }
-      if (tid == 0) {
-        int routed = 0;
-        for (int r = 0; r < picks; ++r)
-          if (s_idx[r] == s_idx[pick]) routed |= 1 << (r / p.k);
-        s_routed = routed;
-      }
-      if (!waited) {
-        wait_prerequisite_grids();                // h comes from the kernel before
-        waited = true;
-      }
-      __syncthreads();
-    }
-    for (int i = tid; i < units * p.M; i += WS_THREADS) {
-      const int tok = i / units, q = i % units;
-      const int st = q >> 4, c8 = q & 15;         // 8-column piece c8 of step st
-      const int sub = c8 / (4 * G4), in = c8 % (4 * G4), tt = in / G4, word = sub * G4 + in % G4;
-      const int k = (s_begin + st) * WS_STEP + c8 * 8;
-      const int unit = ((st * 4 + word) * p.M + tok) * 4 + tt;
-      if constexpr (MODE == WS_DOWN) {
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if ((s_routed >> tok) & 1)
-          ld_h_pairs(p.h + (static_cast<long long>(pick) * p.M + tok) * p.K, k, p.K, hi, lo);
-        reinterpret_cast<uint4*>(xs)[unit] = hi;
-        reinterpret_cast<uint4*>(xs)[x_units + unit] = lo;
-      } else {
-        const T* row = static_cast<const T*>(p.x) + tok * p.x_stride;
-        reinterpret_cast<uint4*>(xs)[unit] = ld_x_pairs<T>(row, k, p.K, (reinterpret_cast<uintptr_t>(row) & 15u) == 0);
-      }
-    }
-    __syncthreads();
-
-    float part_sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto step = [&](const uint4 (&w)[2], int s) {
-      const uint32_t u0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, u1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
-      const int ls = s - s_begin;
-      const int q0 = min(ls * GPS, g_count - 1);
-#pragma unroll
-      for (int gq = 0; gq < GPS; ++gq) {
-        const int q = GPS == 1 ? q0 : min(ls * GPS + gq, g_count - 1);
-        const uint32_t o0 = zo[r0 * sc_pitch + q], o1 = zo[(r0 + 8) * sc_pitch + q];
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = gq * G4; i < (gq + 1) * G4; ++i) {
-          const uint32_t p0 = w4_pair<W>(u0[i], 0, o0), p1 = w4_pair<W>(u0[i], 1, o0), p2 = w4_pair<W>(u0[i], 2, o0),
-                         p3 = w4_pair<W>(u0[i], 3, o0);
-          const uint32_t q0_ = w4_pair<W>(u1[i], 0, o1), q1_ = w4_pair<W>(u1[i], 1, o1), q2_ = w4_pair<W>(u1[i], 2, o1),
-                         q3_ = w4_pair<W>(u1[i], 3, o1);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (g < p.M) x = reinterpret_cast<const uint4*>(xs)[nb * x_units + ((ls * 4 + i) * p.M + g) * 4 + t];
-            mma16816<W>(acc, p0, q0_, p1, q1_, x.x, x.y);
-            mma16816<W>(acc, p2, q2_, p3, q3_, x.z, x.w);
-          }
+      if (s + d < n) {
+        const uint32_t u0[4] = {buf[d][0].x, buf[d][0].y, buf[d][0].z, buf[d][0].w};
+        const uint32_t u1[4] = {buf[d][1].x, buf[d][1].y, buf[d][1].z, buf[d][1].w};
+        if (s + d + WS_DEPTH < n) {
+          buf[d][0] = ld_codes<G4, ALIGNED>(c0, a + s + d + WS_DEPTH, t, pitch);
+          buf[d][1] = ld_codes<G4, ALIGNED>(c1, a + s + d + WS_DEPTH, t, pitch);
         }
-        const float f0 = sc[r0 * sc_pitch + q], f1 = sc[(r0 + 8) * sc_pitch + q];
-        part_sum[0] = fmaf(f0, acc[0], part_sum[0]);
-        part_sum[1] = fmaf(f0, acc[1], part_sum[1]);
-        part_sum[2] = fmaf(f1, acc[2], part_sum[2]);
-        part_sum[3] = fmaf(f1, acc[3], part_sum[3]);
-      }
-    };
-    for (int s = 0; s < n; s += WS_DEPTH) {
+        const uint4 xs[4] = {x[0], x[1], x[2], x[3]};
+        float fa[GPS], fb[GPS];
+        uint32_t oa[GPS], ob[GPS];
 #pragma unroll
-      for (int d = 0; d < WS_DEPTH; ++d)
-        if (s + d < n) {
-          step(buf[d], a + s + d);
-          if (s + d + WS_DEPTH < n) {
-            buf[d][0] = ld_codes<G4, ALIGNED>(c0, a + s + d + WS_DEPTH, t, pitch);
-            buf[d][1] = ld_codes<G4, ALIGNED>(c1, a + s + d + WS_DEPTH, t, pitch);
-          }
+        for (int i = 0; i < GPS; ++i) {
+          fa[i] = s0[i];
+          fb[i] = s1[i];
+          oa[i] = o0[i];
+          ob[i] = o1[i];
         }
-    }
-    if constexpr (MODE == WS_DOWN) {
-      // Weighted sum over the experts; a token that did not pick this one takes nothing, not even 0 * NaN.
-      const int routed = s_routed;
+        if (s + d + 1 < n) side(a + s + d + 1);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int tok = 2 * t + (c & 1);
-        if ((routed >> tok) & 1) total[c] = fmaf(s_wt[tok], part_sum[c], total[c]);
+        for (int q = 0; q < GPS; ++q) {
+          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = q * G4; i < (q + 1) * G4; ++i) {
+            mma16816<T>(acc, w4_pair<T>(u0[i], 0, oa[q]), w4_pair<T>(u1[i], 0, ob[q]), w4_pair<T>(u0[i], 1, oa[q]),
+                        w4_pair<T>(u1[i], 1, ob[q]), xs[i].x, xs[i].y);
+            mma16816<T>(acc, w4_pair<T>(u0[i], 2, oa[q]), w4_pair<T>(u1[i], 2, ob[q]), w4_pair<T>(u0[i], 3, oa[q]),
+                        w4_pair<T>(u1[i], 3, ob[q]), xs[i].z, xs[i].w);
+          }
+          total[0] = fmaf(fa[q], acc[0], total[0]);
+          total[1] = fmaf(fa[q], acc[1], total[1]);
+          total[2] = fmaf(fb[q], acc[2], total[2]);
+          total[3] = fmaf(fb[q], acc[3], total[3]);
+        }
       }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) total[c] += part_sum[c];
-    }
   }
-
-  if constexpr (MODE == WS_DOWN)
-    if (!waited) wait_prerequisite_grids();       // this grid ends after the one before it, with items or without
-
-  // Sum of the cluster's parts, in rank and half order.
-  red[wk][r0][2 * t] = total[0];
-  red[wk][r0][2 * t + 1] = total[1];
-  red[wk][r0 + 8][2 * t] = total[2];
-  red[wk][r0 + 8][2 * t + 1] = total[3];
-  if (S > 1) cluster_sync_all(); else __syncthreads();
-  const uint32_t red_at = smem_u32(&red[0][0][0]);
-  auto sum_at = [&](int row, int tok) {
-    float v = 0.0f;
-    for (int r = 0; r < S; ++r) {
-      const uint32_t base = S > 1 ? cluster_map(red_at, r) : red_at;
+  *reinterpret_cast<float2*>(&red[warp][g][2 * t]) = make_float2(total[0], total[1]);
+  *reinterpret_cast<float2*>(&red[warp][g + 8][2 * t]) = make_float2(total[2], total[3]);
+  __syncthreads();
+  const int row = threadIdx.x % WS_ROWS, tok = threadIdx.x / WS_ROWS;
+  if (tok < p.M && n0 + row < p.N) {
+    float v = red[0][row][tok];
 #pragma unroll
-      for (int q = 0; q < WS_WK; ++q) {
-        float x;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(base + ((q * WS_ROWS + row) * WS_TOK + tok) * 4) : "memory");
-        v += x;
-      }
-    }
-    return v;
-  };
-  if constexpr (MODE == WS_UP) {
-    const int routed = s_routed;
-    for (int i = rank * WS_THREADS + tid; i < WS_ROWS / 2 * WS_TOK; i += S * WS_THREADS) {
-      const int c = i % (WS_ROWS / 2), tok = i / (WS_ROWS / 2), row = (c >> 3) * 16 + (c & 7);
-      const int col = tile * (WS_ROWS / 2) + c;
-      if (tok < p.M && col < p.N && ((routed >> tok) & 1)) {
-        const float u1 = sum_at(row, tok), u2 = sum_at(row + 8, tok);
-        p.h[(static_cast<long long>(slot) * p.M + tok) * p.N + col] = u1 * (u2 / (1.0f + expf(-u2)));
-      }
-    }
-  } else {
-    for (int i = rank * WS_THREADS + tid; i < WS_ROWS * WS_TOK; i += S * WS_THREADS) {
-      const int row = i % WS_ROWS, tok = i / WS_ROWS, col = tile * WS_ROWS + row;
-      if (tok < p.M && col < p.N) static_cast<T*>(p.out)[static_cast<long long>(tok) * p.N + col] = from_f32<T>(sum_at(row, tok));
-    }
+    for (int w = 1; w < WS_WARPS; ++w) v += red[w][row][tok];
+    static_cast<T*>(p.out)[static_cast<long long>(tok) * p.N + n0 + row] = from_f32<T>(v);
   }
-  if (S > 1) cluster_sync_all();                  // no block ends while another reads its sums
 }
 
-// One launch of a cluster of S blocks per row tile (and per slot).
-template <typename T, int MODE>
-inline cudaError_t launch_w4_stream(StreamArgs a, int cluster, int slots, bool programmatic, cudaStream_t st) {
-  const int per = MODE == WS_UP ? WS_ROWS / 2 : WS_ROWS;
-  cudaLaunchConfig_t cfg{};
-  a.cluster = cluster;
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(a.N) + per - 1) / per * cluster), static_cast<unsigned>(slots));
-  cfg.blockDim = dim3(WS_THREADS);
-  cfg.dynamicSmemBytes = ws_smem(MODE, a.M, a.spp, a.w.group);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = programmatic ? 2 : 1;
+template <typename T>
+inline cudaError_t launch_w4_stream(const StreamArgs& a, cudaStream_t st) {
   const bool aligned = ((a.K + 1) / 2) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.w.codes) & 15u) == 0;
-  auto go = [&](auto kernel) -> cudaError_t {
-    // Above 48 KB the size has to be allowed first; a no-op after the first call.
-    if (cfg.dynamicSmemBytes > 40 * 1024)
-      if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes)))
-        return e;
-    return cudaLaunchKernelEx(&cfg, kernel, a);
-  };
+  const unsigned grid = (static_cast<unsigned>(a.N) + WS_ROWS - 1) / WS_ROWS;
+  auto go = [&](auto kernel) { kernel<<<grid, WS_THREADS, 0, st>>>(a); };
   switch (a.w.group) {
-    case 128: return aligned ? go(w4_stream_kernel<T, 4, MODE, true>) : go(w4_stream_kernel<T, 4, MODE, false>);
-    case 64: return aligned ? go(w4_stream_kernel<T, 2, MODE, true>) : go(w4_stream_kernel<T, 2, MODE, false>);
-    default: return aligned ? go(w4_stream_kernel<T, 1, MODE, true>) : go(w4_stream_kernel<T, 1, MODE, false>);
+    case 128: aligned ? go(w4_stream_kernel<T, 4, true>) : go(w4_stream_kernel<T, 4, false>); break;
+    case 64: aligned ? go(w4_stream_kernel<T, 2, true>) : go(w4_stream_kernel<T, 2, false>); break;
+    default: aligned ? go(w4_stream_kernel<T, 1, true>) : go(w4_stream_kernel<T, 1, false>); break;
   }
+  return cudaGetLastError();
 }
 
 }  // namespace moe
