@@ -92,17 +92,17 @@ __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   return v;
 }
 
-// The four words of one step that thread t of a row's four holds. G4 = group / 32 words per group.
-// Word i of the step: columns (i / G4) * group + t * group / 4 + (i % G4) * 8 .. + 8.
-template <int G4, bool ALIGNED>
-__device__ __forceinline__ uint4 ld_codes(const uint8_t* row, int step, int t, int pitch) {
-  const int base = step * (WS_STEP / 2);
+// The four words of one step that thread t of a row's four holds; `row` is the row's code byte of the step's first column
+// plus 4 G4 t. G4 = group / 32 words per group: word i holds columns (i / G4) * group + t * group / 4 + (i % G4) * 8 .. + 8.
+// `left`: bytes of the row from `row` on. FULL: the whole step lies inside the row.
+template <int G4, bool ALIGNED, bool FULL>
+__device__ __forceinline__ uint4 ld_codes(const uint8_t* row, int left) {
   uint32_t v[4] = {0u, 0u, 0u, 0u};
   if constexpr (ALIGNED) {
 #pragma unroll
     for (int s = 0; s < 4 / G4; ++s) {
-      const int o = base + s * (16 * G4) + t * (4 * G4);
-      if (o < pitch) {
+      const int o = s * (16 * G4);
+      if (FULL || o < left) {
         if constexpr (G4 == 4) {
           return ld_stream_v4(row + o);
         } else if constexpr (G4 == 2) {
@@ -117,8 +117,8 @@ __device__ __forceinline__ uint4 ld_codes(const uint8_t* row, int step, int t, i
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int o = base + (i / G4) * (16 * G4) + t * (4 * G4) + (i % G4) * 4;
-      v[i] = ld_u32_any(row + o, pitch - o);
+      const int o = (i / G4) * (16 * G4) + (i % G4) * 4;
+      v[i] = ld_u32_any(row + o, left - o);
     }
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
@@ -155,36 +155,64 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
   const int a = warp * per, n = min(steps, a + per) - a;            // this warp's steps (n may be 0 or less)
   const int n0 = blockIdx.x * WS_ROWS;
   const long long r0 = min(n0 + g, p.N - 1), r1 = min(n0 + g + 8, p.N - 1);   // rows past N repeat the last one
-  const uint8_t *c0 = p.w.codes + r0 * pitch, *c1 = p.w.codes + r1 * pitch;
   const T *f0 = static_cast<const T*>(p.w.scale) + r0 * groups, *f1 = static_cast<const T*>(p.w.scale) + r1 * groups;
   const uint8_t *z0 = p.w.zero ? p.w.zero + r0 * groups : nullptr, *z1 = p.w.zero ? p.w.zero + r1 * groups : nullptr;
   const T* xrow = static_cast<const T*>(p.x) + min(g, p.M - 1) * p.x_stride;
   const bool vec = (reinterpret_cast<uintptr_t>(xrow) & 15u) == 0;
 
+  // Steps that lie wholly inside the rows are read without a check per load (all of them where K is a multiple of 128 and
+  // the rows allow 16-byte loads).
+  const int whole = ALIGNED && vec ? p.K / WS_STEP : 0;
+  const uint8_t *c0 = p.w.codes + r0 * pitch + 4 * G4 * t, *c1 = p.w.codes + r1 * pitch + 4 * G4 * t;
+  const T* xt = xrow + 8 * G4 * t;
   uint4 buf[WS_DEPTH][2];
+  auto codes = [&](int step, uint4 (&o)[2]) {
+    const long long at = static_cast<long long>(step) * (WS_STEP / 2);
+    const int left = pitch - static_cast<int>(at) - 4 * G4 * t;
+    if (step < whole) {
+      o[0] = ld_codes<G4, ALIGNED, true>(c0 + at, left);
+      o[1] = ld_codes<G4, ALIGNED, true>(c1 + at, left);
+    } else {
+      o[0] = ld_codes<G4, ALIGNED, false>(c0 + at, left);
+      o[1] = ld_codes<G4, ALIGNED, false>(c1 + at, left);
+    }
+  };
 #pragma unroll
   for (int d = 0; d < WS_DEPTH; ++d)
-    if (d < n) {
-      buf[d][0] = ld_codes<G4, ALIGNED>(c0, a + d, t, pitch);
-      buf[d][1] = ld_codes<G4, ALIGNED>(c1, a + d, t, pitch);
-    }
+    if (d < n) codes(a + d, buf[d]);
   // One step ahead: activations, scales and zero points.
   uint4 x[4];
   float s0[GPS], s1[GPS];
   uint32_t o0[GPS], o1[GPS];
-  auto side = [&](int step) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = step * WS_STEP + (i / G4) * (32 * G4) + t * (8 * G4) + (i % G4) * 8;
-      x[i] = g < p.M ? ld_x_pairs<T>(xrow, k, p.K, vec) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < 4; ++i) x[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < GPS; ++i) o0[i] = o1[i] = w4_offset<T>(8);
+  auto side = [&](int step) {
+    const int k0 = step * WS_STEP;
+    if (g < p.M) {
+      if (step < whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(xt + k0 + (i / G4) * (32 * G4) + (i % G4) * 8));
+          x[i] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                            __byte_perm(v.y, v.w, 0x7632));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = ld_x_pairs<T>(xrow, k0 + (i / G4) * (32 * G4) + t * (8 * G4) + (i % G4) * 8, p.K, vec);
+      }
     }
 #pragma unroll
     for (int i = 0; i < GPS; ++i) {
-      const int q = min(step * GPS + i, groups - 1);
+      const int q = step < whole ? step * GPS + i : min(step * GPS + i, groups - 1);
       s0[i] = to_f32(f0[q]);
       s1[i] = to_f32(f1[q]);
-      o0[i] = w4_offset<T>(z0 ? __ldg(z0 + q) & 15 : 8);
-      o1[i] = w4_offset<T>(z1 ? __ldg(z1 + q) & 15 : 8);
+      if (z0) {
+        o0[i] = w4_offset<T>(__ldg(z0 + q) & 15);
+        o1[i] = w4_offset<T>(__ldg(z1 + q) & 15);
+      }
     }
   };
   float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -195,10 +223,7 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
       if (s + d < n) {
         const uint32_t u0[4] = {buf[d][0].x, buf[d][0].y, buf[d][0].z, buf[d][0].w};
         const uint32_t u1[4] = {buf[d][1].x, buf[d][1].y, buf[d][1].z, buf[d][1].w};
-        if (s + d + WS_DEPTH < n) {
-          buf[d][0] = ld_codes<G4, ALIGNED>(c0, a + s + d + WS_DEPTH, t, pitch);
-          buf[d][1] = ld_codes<G4, ALIGNED>(c1, a + s + d + WS_DEPTH, t, pitch);
-        }
+        if (s + d + WS_DEPTH < n) codes(a + s + d + WS_DEPTH, buf[d]);
         const uint4 xs[4] = {x[0], x[1], x[2], x[3]};
         float fa[GPS], fb[GPS];
         uint32_t oa[GPS], ob[GPS];
