@@ -17,7 +17,6 @@ _synth_cpu = None
 
 c_int, c_float, c_size_t, c_void_p, c_uint64 = (ctypes.c_int, ctypes.c_float, ctypes.c_size_t,
                                                  ctypes.c_void_p, ctypes.c_uint64)
-c_longlong = ctypes.c_longlong
 c_int_p = ctypes.POINTER(ctypes.c_int)
 c_size_t_p = ctypes.POINTER(ctypes.c_size_t)
 
@@ -66,17 +65,13 @@ CUDA_SIGNATURES = {
     "moe_gate_packed_bytes": (c_size_t, []),
     "moe_pack_gate": (c_int, [c_void_p, c_void_p, c_void_p]),
     "moe_gate_quantize": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "moe_route_experts": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
-                                  c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),
-    "moe_route_experts_backward": (c_int, [c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int, c_int, c_int,
-                                           c_int, c_int, c_float, c_void_p, c_void_p]),
+    # These take a struct, handed over as its bytes (experts.py packs them).
+    "moe_route_experts": (c_int, [ctypes.c_char_p]),
+    "moe_route_experts_backward": (c_int, [ctypes.c_char_p]),
     "moe_linear_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
-    "moe_linear_w4": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                              c_void_p, c_void_p, c_size_t, c_void_p]),
+    "moe_linear_w4": (c_int, [ctypes.c_char_p]),
     "moe_experts_w4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
-    "moe_experts_w4": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                               c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                               c_void_p, c_void_p, c_size_t, c_void_p]),
+    "moe_experts_w4": (c_int, [ctypes.c_char_p]),
     "moe_synth_logits": (c_int, [c_void_p, c_uint64, c_int, c_int, c_void_p, c_void_p]),
     "moe_synth_bias": (c_int, [c_void_p, c_uint64, c_int, c_float, c_void_p, c_int, c_float,
                                c_void_p, c_void_p]),

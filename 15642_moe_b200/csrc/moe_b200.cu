@@ -801,7 +801,11 @@ int launch_w4_mma_nt(DeviceInfo* d, const WmArgs& a, const void* x, long long x_
     if (int rc = w4_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w.codes, dims, strides, box, &maps.codes)) return rc;
   }
   const CUtensorMapDataType t = MODE != WS_DOWN && std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  for (int i = 0; 16 * (i + 1) <= NT; ++i) {
+  // linear_w4 has tiles of two sizes at most; an expert's can have any.
+  const int tiles_m = MODE == WS_LINEAR ? (a.M + NT - 1) / NT : 1;
+  const int box0 = MODE == WS_LINEAR ? (a.M / tiles_m + 15) / 16 - 1 : 0;
+  const int box1 = MODE == WS_LINEAR ? ((a.M + tiles_m - 1) / tiles_m + 15) / 16 - 1 : NT / 16 - 1;
+  for (int i = box0; i <= box1; ++i) {
     const long long pitch = round_up(a.K, 64) * 2ll, rows = x_rows / TERMS;
     const long long dims[4] = {64, rows, TERMS, pitch / 128}, strides[3] = {pitch, pitch * rows, 128};
     const int box[4] = {64, 16 * (i + 1), TERMS, WmShape<NT, TERMS, 128>::B_COLS / 64};
@@ -833,7 +837,7 @@ int w4_tma_codes(DeviceInfo* d, const uint8_t* codes, long long rows, int K, uin
   *out = codes;
   if (w4_rows_aligned(codes, K)) return MOE_OK;
   const int bytes = w4_bytes(K), pitch = round_up(bytes, 16);
-  pad_codes_kernel<<<grid_for(static_cast<size_t>(rows) * (pitch / 4), 256, d->num_sms * 16), 256, 0, st>>>(codes, rows, bytes, pitch, copy);
+  pad_codes_kernel<<<grid_for(static_cast<size_t>(rows) * (pitch / 4), 256, d->num_sms * 16), 256, 0, st>>>(codes, rows, bytes, copy);
   *out = copy;
   return cuda_check(cudaGetLastError(), "pad_codes launch");
 }
@@ -841,7 +845,7 @@ int w4_tma_codes(DeviceInfo* d, const uint8_t* codes, long long rows, int K, uin
 template <typename T>
 int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Matrix& w, int M, int N, int K, void* out, void* workspace,
                    cudaStream_t st) {
-  if (M <= WS_TOK) {
+  if (M <= WS_MAX_TOK) {
     const StreamArgs a{x, x_stride, w, M, N, K, out};
     return cuda_check(launch_w4_stream<T>(a, st), "linear_w4 launch");
   }
@@ -849,9 +853,12 @@ int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Mat
   uint8_t* W = static_cast<uint8_t*>(workspace);
   WmArgs a{};
   a.w = w;
-  if (int rc = w4_tma_codes(d, w.codes, N, K, W + ws.codes, &a.w.codes, st)) return rc;
-  pair_rows_kernel<T><<<dim3((round_up(K, 64) / 8 + 255) / 256, M), 256, 0, st>>>(
-      static_cast<const T*>(x), x_stride, M, K, reinterpret_cast<T*>(W + ws.x));
+  const bool copy = !w4_rows_aligned(w.codes, K);
+  const int row_blocks = static_cast<int>((static_cast<long long>(M) * (round_up(K, 64) / 8) + 255) / 256);
+  const int code_blocks = copy ? grid_for(static_cast<size_t>(N) * (round_up(w4_bytes(K), 16) / 4), 256, d->num_sms * 16) : 0;
+  linear_w4_layout_kernel<T><<<row_blocks + code_blocks, 256, 0, st>>>(static_cast<const T*>(x), x_stride, M, K, reinterpret_cast<T*>(W + ws.x),
+                                                                      row_blocks, w.codes, N, W + ws.codes);
+  if (copy) a.w.codes = W + ws.codes;
   a.E = 1;
   a.N = N;
   a.K = K;
@@ -919,9 +926,9 @@ int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W
 
 extern "C" {
 
-int moe_route_experts(const void* logits, int dtype, long long row_stride, const float* bias, int T, int E, int top_k,
-                      int score, int n_group, int topk_group, int group_score, int renormalize, float scale, int* idx,
-                      float* w, void* stream) {
+int moe_route_experts(const moe_route_experts_args* args) {
+  if (args == nullptr) return fail(MOE_ERR_INVALID, "moe_route_experts: null pointer argument");
+  const auto [logits, bias, idx, w, stream, row_stride, dtype, T, E, top_k, score, n_group, topk_group, group_score, renormalize, scale] = *args;
   if (dtype < MOE_F32 || dtype > MOE_F16) return fail(MOE_ERR_INVALID, "moe_route_experts: bad dtype");
   if (T < 0 || E < 1 || E > RX_MAX_E) return fail(MOE_ERR_INVALID, "moe_route_experts: logits must be [T, E] with 1 <= E <= 1024");
   if (n_group < 1 || n_group > RX_MAX_GROUPS || E % n_group != 0)
@@ -944,9 +951,9 @@ int moe_route_experts(const void* logits, int dtype, long long row_stride, const
   return cuda_check(cudaGetLastError(), "route_experts launch");
 }
 
-int moe_route_experts_backward(const float* grad_w, const void* logits, int dtype, long long row_stride, const int* idx,
-                               int T, int E, int top_k, int score, int renormalize, float scale, void* grad_logits,
-                               void* stream) {
+int moe_route_experts_backward(const moe_route_experts_backward_args* args) {
+  if (args == nullptr) return fail(MOE_ERR_INVALID, "moe_route_experts_backward: null pointer argument");
+  const auto [grad_w, logits, idx, grad_logits, stream, row_stride, dtype, T, E, top_k, score, renormalize, scale] = *args;
   if (dtype < MOE_F32 || dtype > MOE_F16) return fail(MOE_ERR_INVALID, "moe_route_experts_backward: bad dtype");
   if (T < 0 || E < 1 || E > RX_MAX_E)
     return fail(MOE_ERR_INVALID, "moe_route_experts_backward: logits must be [T, E] with 1 <= E <= 1024");
@@ -964,21 +971,23 @@ int moe_route_experts_backward(const float* grad_w, const void* logits, int dtyp
 }
 
 size_t moe_linear_w4_workspace_bytes(int M, int N, int K) {
-  if (M <= WS_TOK || N < 1 || K < 1) return 0;
+  if (M <= WS_MAX_TOK || N < 1 || K < 1) return 0;
   return make_linear_w4_ws(M, N, K).total;
 }
 
-int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* codes, const void* scale, const void* zero,
-                  int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+int moe_linear_w4(const moe_linear_w4_args* args) {
+  if (args == nullptr) return fail(MOE_ERR_INVALID, "moe_linear_w4: null pointer argument");
+  const auto [x, codes, scale, zero, out, workspace, stream, x_stride, workspace_bytes, dtype, group, M, N, K] = *args;
   if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be bf16 or f16");
   if (M < 0 || N < 1 || K < 1) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be [M, K] and W [N, K]");
-  if (M > WM_MAX_ROWS) return fail(MOE_ERR_INVALID, "moe_linear_w4: M must be at most 65535");
+  if (M > WM_MAX_ROWS || static_cast<long long>(M) * round_up(K, 64) > 0x7FFFFFFFll)
+    return fail(MOE_ERR_INVALID, "moe_linear_w4: M must be at most 65535, and x have less than 2^31 elements");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_linear_w4: group must be 32, 64 or 128");
   if (M == 0) return MOE_OK;
   if (!x || !codes || !scale || !out) return fail(MOE_ERR_INVALID, "moe_linear_w4: null pointer argument");
   const W4Matrix w{static_cast<const uint8_t*>(codes), scale, static_cast<const uint8_t*>(zero), group};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M > WS_TOK) {
+  if (M > WS_MAX_TOK) {
     const size_t need = moe_linear_w4_workspace_bytes(M, N, K);
     if (workspace == nullptr || workspace_bytes < need)
       return fail(MOE_ERR_WORKSPACE, "moe_linear_w4: workspace too small: need " + std::to_string(need) + " bytes");
@@ -996,10 +1005,10 @@ size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I) {
   return make_experts_w4_ws(T, top_k, E, H, I).total;
 }
 
-int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx, const float* w, const void* w13,
-                   const void* w13_scale, const void* w13_zero, const void* w2, const void* w2_scale,
-                   const void* w2_zero, int group, int T, int top_k, int E, int local_offset, int H, int I, void* out,
-                   void* workspace, size_t workspace_bytes, void* stream) {
+int moe_experts_w4(const moe_experts_w4_args* args) {
+  if (args == nullptr) return fail(MOE_ERR_INVALID, "moe_experts_w4: null pointer argument");
+  const auto [x, idx, w, w13, w13_scale, w13_zero, w2, w2_scale, w2_zero, out, workspace, stream, x_stride, workspace_bytes, dtype, group, T,
+              top_k, E, local_offset, H, I] = *args;
   if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_experts_w4: x must be bf16 or f16");
   if (T < 0 || T > WM_MAX_ROWS) return fail(MOE_ERR_INVALID, "moe_experts_w4: T must be 0 to 65535");
   if (top_k < 1 || top_k > RX_MAX_K) return fail(MOE_ERR_INVALID, "moe_experts_w4: top_k must be 1 to 32");

@@ -624,25 +624,33 @@ __device__ __forceinline__ uint4 ld_pairs(const T* row, int k, int K) {
   return *reinterpret_cast<const uint4*>(o);
 }
 
-// Rows of x in pair order, columns padded with zeros to a multiple of 64. One warp per row and stretch of columns.
-template <typename T>
-__global__ void __launch_bounds__(256) pair_rows_kernel(const T* x, long long x_stride, int M, int K, T* out) {
-  allow_dependent_launch();
-  const int per = (K + 63) / 64 * 8;
-  const long long m = blockIdx.y;
-  for (int c = blockIdx.x * 256 + threadIdx.x; c < per; c += gridDim.x * 256)
-    reinterpret_cast<uint4*>(out)[m * per + c] = ld_pairs(x + m * x_stride, c * 8, K);
-}
-
-// Codes with a row pitch of a multiple of 16 bytes, for shapes whose own rows do not allow TMA.
-__global__ void __launch_bounds__(256) pad_codes_kernel(const uint8_t* codes, long long rows, int bytes, int pitch, uint8_t* out) {
-  const long long n = rows * (pitch / 4);
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const long long r = i / (pitch / 4);
-    const int o = static_cast<int>(i % (pitch / 4)) * 4;
+// Codes with a row pitch of a multiple of 16 bytes, for shapes whose own rows do not allow TMA: words i, i + stride, ...
+__device__ __forceinline__ void pad_codes(const uint8_t* codes, long long rows, int bytes, uint8_t* out, long long i, long long stride) {
+  const int words = (bytes + 15) / 16 * 4;
+  for (const long long n = rows * words; i < n; i += stride) {
+    const long long r = i / words;
+    const int o = static_cast<int>(i % words) * 4;
     uint32_t v = ld_u32_any(codes + r * bytes + o, bytes - o);
     if (bytes - o < 4) v = bytes > o ? v & ((1u << (8 * (bytes - o))) - 1u) : 0u;
     reinterpret_cast<uint32_t*>(out)[i] = v;
+  }
+}
+__global__ void __launch_bounds__(256) pad_codes_kernel(const uint8_t* codes, long long rows, int bytes, uint8_t* out) {
+  pad_codes(codes, rows, bytes, out, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
+}
+
+// What linear_w4 lays out for the product, in one launch: rows of x in pair order, columns padded with zeros to a multiple
+// of 64 (the first `row_blocks` blocks, 256 pieces of 8 columns each), and the codes' copy where one is needed.
+template <typename T>
+__global__ void __launch_bounds__(256) linear_w4_layout_kernel(const T* x, long long x_stride, int M, int K, T* out, int row_blocks,
+                                                               const uint8_t* codes, int N, uint8_t* copy) {
+  allow_dependent_launch();
+  const int per = (K + 63) / 64 * 8, b = blockIdx.x;
+  if (b < row_blocks) {
+    const int i = b * 256 + threadIdx.x;                  // M * per < 2^31 / 8: at most 65535 rows of 2^31 / 65535 columns
+    if (i < M * per) reinterpret_cast<uint4*>(out)[i] = ld_pairs(x + static_cast<long long>(i / per) * x_stride, i % per * 8, K);
+  } else {
+    pad_codes(codes, N, (K + 1) / 2, copy, (b - row_blocks) * 256ll + threadIdx.x, (gridDim.x - row_blocks) * 256ll);
   }
 }
 

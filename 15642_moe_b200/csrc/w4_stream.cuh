@@ -1,8 +1,8 @@
 /*
- * linear_w4 for up to 8 tokens, in one launch: the weights are read once, straight from global memory into matrix
+ * linear_w4 for up to 16 tokens, in one launch: the weights are read once, straight from global memory into matrix
  * fragments.
  *
- *   mma m16n8k16: A = 16 weight rows x 16 columns, B = 16 columns x 8 tokens, fp32 accumulators.
+ *   mma m16n8k16: A = 16 weight rows x 16 columns, B = 16 columns x 8 tokens, fp32 accumulators; one or two B per A.
  *
  * A thread holds, of rows g and g + 8 of a tile, the codes at a few places; which columns those are is free as long as A
  * and B agree. Thread t of a row's four takes group / 4 neighbouring columns of each group (one 16-, 8- or 4-byte load); a
@@ -11,8 +11,8 @@
  * fp32: no weight is rounded.
  *
  * Split: a block has one tile of 16 rows, its 8 warps an eighth of the columns each; their sums meet in shared memory in
- * warp order, so results repeat bit for bit. Nothing is staged: a warp alone uses its columns of x. 4 steps of 128 columns
- * are in flight per warp (4 KB).
+ * warp order, so results repeat bit for bit. Nothing is staged: a warp alone uses its columns of x. 1 to 4 steps of 128
+ * columns are in flight per warp (1 KB each).
  */
 #pragma once
 #include "gate.cuh"
@@ -25,8 +25,8 @@ namespace moe {
 constexpr int WS_WARPS = 8, WS_THREADS = 32 * WS_WARPS;
 constexpr int WS_ROWS = 16;                     // weight rows per block
 constexpr int WS_TOK = 8;                       // tokens per mma
+constexpr int WS_MAX_TOK = 16;                  // tokens that this kernel takes: two mma per fragment of weights
 constexpr int WS_STEP = 128;                    // columns per step
-constexpr int WS_DEPTH = 4;                     // steps in flight per warp
 
 enum { WS_LINEAR = 0, WS_UP = 1, WS_DOWN = 2 };  // which product a kernel computes: linear_w4, the experts' first, second
 
@@ -34,7 +34,7 @@ struct StreamArgs {
   const void* x;           // [M, K]
   long long x_stride;
   W4Matrix w;
-  int M, N, K;             // tokens (<= 8), output columns, reduction length
+  int M, N, K;             // tokens (<= 16), output columns, reduction length
   void* out;               // [M, N]
 };
 
@@ -133,8 +133,22 @@ __device__ __forceinline__ uint32_t pack2(T a, T b) {
 // 8 neighbouring activations from column k on (0 past K) as the pairs (0,4), (1,5), (2,6), (3,7).
 template <typename T>
 __device__ __forceinline__ uint4 ld_x_pairs(const T* row, int k, int K, bool vec) {
-  if (vec && k + 8 <= K) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (k + 8 <= K) {
+    uint4 v;
+    if (vec) {
+      v = __ldg(reinterpret_cast<const uint4*>(row + k));
+    } else {
+      // Aligned words that hold a wanted value, shifted together where the row starts in the middle of one.
+      const uintptr_t at = reinterpret_cast<uintptr_t>(row + k);
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+      const int sh = static_cast<int>(at & 2) * 8;
+      uint32_t u[5];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = __ldg(w + i);
+      u[4] = sh ? __ldg(w + 4) : 0u;
+      v = make_uint4(__funnelshift_r(u[0], u[1], sh), __funnelshift_r(u[1], u[2], sh), __funnelshift_r(u[2], u[3], sh),
+                     __funnelshift_r(u[3], u[4], sh));
+    }
     return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                       __byte_perm(v.y, v.w, 0x7632));
   }
@@ -144,10 +158,13 @@ __device__ __forceinline__ uint4 ld_x_pairs(const T* row, int k, int K, bool vec
   return make_uint4(pack2(e[0], e[4]), pack2(e[1], e[5]), pack2(e[2], e[6]), pack2(e[3], e[7]));
 }
 
-template <typename T, int G4, bool ALIGNED>
+template <typename T, int G4, bool ALIGNED, int NB>
 __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_constant__ StreamArgs p) {
   constexpr int GPS = 4 / G4;                    // groups per step
-  __shared__ float red[WS_WARPS][WS_ROWS][WS_TOK];
+  // Steps in flight per warp, which is also how often the step's code is unrolled: the long ones (many groups, byte-wise
+  // addresses) would spend more time fetching instructions than they win.
+  constexpr int DEPTH = !ALIGNED ? 1 : G4 == 4 ? 4 : 2;
+  __shared__ float red[WS_WARPS][WS_ROWS][NB * WS_TOK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pitch = (p.K + 1) / 2, steps = (p.K + WS_STEP - 1) / WS_STEP;
   const int groups = (p.K + p.w.group - 1) / p.w.group;
@@ -157,15 +174,19 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
   const long long r0 = min(n0 + g, p.N - 1), r1 = min(n0 + g + 8, p.N - 1);   // rows past N repeat the last one
   const T *f0 = static_cast<const T*>(p.w.scale) + r0 * groups, *f1 = static_cast<const T*>(p.w.scale) + r1 * groups;
   const uint8_t *z0 = p.w.zero ? p.w.zero + r0 * groups : nullptr, *z1 = p.w.zero ? p.w.zero + r1 * groups : nullptr;
-  const T* xrow = static_cast<const T*>(p.x) + min(g, p.M - 1) * p.x_stride;
-  const bool vec = (reinterpret_cast<uintptr_t>(xrow) & 15u) == 0;
+  const T* xrow[NB];
+  bool vec = true;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    xrow[b] = static_cast<const T*>(p.x) + min(b * WS_TOK + g, p.M - 1) * p.x_stride;
+    vec = vec && (reinterpret_cast<uintptr_t>(xrow[b]) & 15u) == 0;
+  }
 
   // Steps that lie wholly inside the rows are read without a check per load (all of them where K is a multiple of 128 and
   // the rows allow 16-byte loads).
   const int whole = ALIGNED && vec ? p.K / WS_STEP : 0;
   const uint8_t *c0 = p.w.codes + r0 * pitch + 4 * G4 * t, *c1 = p.w.codes + r1 * pitch + 4 * G4 * t;
-  const T* xt = xrow + 8 * G4 * t;
-  uint4 buf[WS_DEPTH][2];
+  uint4 buf[DEPTH][2];
   auto codes = [&](int step, uint4 (&o)[2]) {
     const long long at = static_cast<long long>(step) * (WS_STEP / 2);
     const int left = pitch - static_cast<int>(at) - 4 * G4 * t;
@@ -178,32 +199,35 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
     }
   };
 #pragma unroll
-  for (int d = 0; d < WS_DEPTH; ++d)
+  for (int d = 0; d < DEPTH; ++d)
     if (d < n) codes(a + d, buf[d]);
   // One step ahead: activations, scales and zero points.
-  uint4 x[4];
+  uint4 x[NB][4];
   float s0[GPS], s1[GPS];
   uint32_t o0[GPS], o1[GPS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < 4 * NB; ++i) x[i / 4][i % 4] = make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int i = 0; i < GPS; ++i) o0[i] = o1[i] = w4_offset<T>(8);
   auto side = [&](int step) {
     const int k0 = step * WS_STEP;
-    if (g < p.M) {
-      if (step < whole) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(xt + k0 + (i / G4) * (32 * G4) + (i % G4) * 8));
-          x[i] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                            __byte_perm(v.y, v.w, 0x7632));
+    for (int b = 0; b < NB; ++b)
+      if (b * WS_TOK + g < p.M) {
+        if (step < whole) {
+          const T* xt = xrow[b] + k0 + 8 * G4 * t;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(xt + (i / G4) * (32 * G4) + (i % G4) * 8));
+            x[b][i] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                                 __byte_perm(v.y, v.w, 0x7632));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[b][i] = ld_x_pairs<T>(xrow[b], k0 + (i / G4) * (32 * G4) + t * (8 * G4) + (i % G4) * 8, p.K, vec);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = ld_x_pairs<T>(xrow, k0 + (i / G4) * (32 * G4) + t * (8 * G4) + (i % G4) * 8, p.K, vec);
       }
-    }
 #pragma unroll
     for (int i = 0; i < GPS; ++i) {
       const int q = step < whole ? step * GPS + i : min(step * GPS + i, groups - 1);
@@ -215,16 +239,20 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
       }
     }
   };
-  float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (n > 0) side(a);
-  for (int s = 0; s < n; s += WS_DEPTH) {
+  float total[NB][4];
 #pragma unroll
-    for (int d = 0; d < WS_DEPTH; ++d)
+  for (int i = 0; i < 4 * NB; ++i) total[i / 4][i % 4] = 0.0f;
+  if (n > 0) side(a);
+  for (int s = 0; s < n; s += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
       if (s + d < n) {
         const uint32_t u0[4] = {buf[d][0].x, buf[d][0].y, buf[d][0].z, buf[d][0].w};
         const uint32_t u1[4] = {buf[d][1].x, buf[d][1].y, buf[d][1].z, buf[d][1].w};
-        if (s + d + WS_DEPTH < n) codes(a + s + d + WS_DEPTH, buf[d]);
-        const uint4 xs[4] = {x[0], x[1], x[2], x[3]};
+        if (s + d + DEPTH < n) codes(a + s + d + DEPTH, buf[d]);
+        uint4 xs[NB][4];
+#pragma unroll
+        for (int i = 0; i < 4 * NB; ++i) xs[i / 4][i % 4] = x[i / 4][i % 4];
         float fa[GPS], fb[GPS];
         uint32_t oa[GPS], ob[GPS];
 #pragma unroll
@@ -237,23 +265,35 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
         if (s + d + 1 < n) side(a + s + d + 1);
 #pragma unroll
         for (int q = 0; q < GPS; ++q) {
-          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          float acc[NB][4];
+#pragma unroll
+          for (int i = 0; i < 4 * NB; ++i) acc[i / 4][i % 4] = 0.0f;
 #pragma unroll
           for (int i = q * G4; i < (q + 1) * G4; ++i) {
-            mma16816<T>(acc, w4_pair<T>(u0[i], 0, oa[q]), w4_pair<T>(u1[i], 0, ob[q]), w4_pair<T>(u0[i], 1, oa[q]),
-                        w4_pair<T>(u1[i], 1, ob[q]), xs[i].x, xs[i].y);
-            mma16816<T>(acc, w4_pair<T>(u0[i], 2, oa[q]), w4_pair<T>(u1[i], 2, ob[q]), w4_pair<T>(u0[i], 3, oa[q]),
-                        w4_pair<T>(u1[i], 3, ob[q]), xs[i].z, xs[i].w);
+            const uint32_t p0 = w4_pair<T>(u0[i], 0, oa[q]), p1 = w4_pair<T>(u0[i], 1, oa[q]), q0 = w4_pair<T>(u1[i], 0, ob[q]),
+                           q1 = w4_pair<T>(u1[i], 1, ob[q]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma16816<T>(acc[b], p0, q0, p1, q1, xs[b][i].x, xs[b][i].y);
+            const uint32_t p2 = w4_pair<T>(u0[i], 2, oa[q]), p3 = w4_pair<T>(u0[i], 3, oa[q]), q2 = w4_pair<T>(u1[i], 2, ob[q]),
+                           q3 = w4_pair<T>(u1[i], 3, ob[q]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma16816<T>(acc[b], p2, q2, p3, q3, xs[b][i].z, xs[b][i].w);
           }
-          total[0] = fmaf(fa[q], acc[0], total[0]);
-          total[1] = fmaf(fa[q], acc[1], total[1]);
-          total[2] = fmaf(fb[q], acc[2], total[2]);
-          total[3] = fmaf(fb[q], acc[3], total[3]);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            total[b][0] = fmaf(fa[q], acc[b][0], total[b][0]);
+            total[b][1] = fmaf(fa[q], acc[b][1], total[b][1]);
+            total[b][2] = fmaf(fb[q], acc[b][2], total[b][2]);
+            total[b][3] = fmaf(fb[q], acc[b][3], total[b][3]);
+          }
         }
       }
   }
-  *reinterpret_cast<float2*>(&red[warp][g][2 * t]) = make_float2(total[0], total[1]);
-  *reinterpret_cast<float2*>(&red[warp][g + 8][2 * t]) = make_float2(total[2], total[3]);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    *reinterpret_cast<float2*>(&red[warp][g][b * WS_TOK + 2 * t]) = make_float2(total[b][0], total[b][1]);
+    *reinterpret_cast<float2*>(&red[warp][g + 8][b * WS_TOK + 2 * t]) = make_float2(total[b][2], total[b][3]);
+  }
   __syncthreads();
   const int row = threadIdx.x % WS_ROWS, tok = threadIdx.x / WS_ROWS;
   if (tok < p.M && n0 + row < p.N) {
@@ -264,17 +304,21 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
   }
 }
 
-template <typename T>
-inline cudaError_t launch_w4_stream(const StreamArgs& a, cudaStream_t st) {
+template <typename T, int NB>
+inline cudaError_t launch_w4_stream_nb(const StreamArgs& a, cudaStream_t st) {
   const bool aligned = ((a.K + 1) / 2) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.w.codes) & 15u) == 0;
   const unsigned grid = (static_cast<unsigned>(a.N) + WS_ROWS - 1) / WS_ROWS;
   auto go = [&](auto kernel) { kernel<<<grid, WS_THREADS, 0, st>>>(a); };
   switch (a.w.group) {
-    case 128: aligned ? go(w4_stream_kernel<T, 4, true>) : go(w4_stream_kernel<T, 4, false>); break;
-    case 64: aligned ? go(w4_stream_kernel<T, 2, true>) : go(w4_stream_kernel<T, 2, false>); break;
-    default: aligned ? go(w4_stream_kernel<T, 1, true>) : go(w4_stream_kernel<T, 1, false>); break;
+    case 128: aligned ? go(w4_stream_kernel<T, 4, true, NB>) : go(w4_stream_kernel<T, 4, false, NB>); break;
+    case 64: aligned ? go(w4_stream_kernel<T, 2, true, NB>) : go(w4_stream_kernel<T, 2, false, NB>); break;
+    default: aligned ? go(w4_stream_kernel<T, 1, true, NB>) : go(w4_stream_kernel<T, 1, false, NB>); break;
   }
   return cudaGetLastError();
+}
+template <typename T>
+inline cudaError_t launch_w4_stream(const StreamArgs& a, cudaStream_t st) {
+  return a.M <= WS_TOK ? launch_w4_stream_nb<T, 1>(a, st) : launch_w4_stream_nb<T, 2>(a, st);
 }
 
 }  // namespace moe

@@ -13,6 +13,7 @@ several experts are stacked in a leading dimension.
 from __future__ import annotations
 
 import functools
+import struct
 
 import torch
 
@@ -38,13 +39,20 @@ def _native_lib():
     return _lib
 
 
-def _call(fn, index: int, *args) -> None:
-    """One C call on device `index` and its current stream."""
+# The argument structs of include/moe_b200.h.
+_ROUTE = struct.Struct("@5Pq9if").pack
+_ROUTE_BACKWARD = struct.Struct("@5Pq6if").pack
+_LINEAR = struct.Struct("@7P2q5i").pack
+_EXPERTS = struct.Struct("@12P2q8i").pack
+
+
+def _call(fn, index: int, args: bytes) -> None:
+    """One C call with device `index` current."""
     if index == torch.cuda.current_device():
-        rc = fn(*args, _current_stream(index))
+        rc = fn(args)
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _current_stream(index))
+            rc = fn(args)
     if rc:
         _native.check(rc)
 
@@ -102,7 +110,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         _fail(f"top_k must be 1 to {MAX_TOP_K} and at most the experts of topk_group groups")
     if n_group > 1 and group_score == "top2" and E // n_group < 2:
         _fail("group_score 'top2' needs two experts per group")
-    index, bias_ptr = logits.get_device(), None
+    index, bias_ptr = logits.get_device(), 0
     if bias is not None:
         if not (bias.dtype == torch.float32 and bias.dim() == 1 and bias.shape[0] == E and bias.is_contiguous()
                 and bias.is_cuda and bias.get_device() == index):
@@ -111,9 +119,10 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     w = logits.new_empty((T, top_k), dtype=torch.float32)
     idx = torch.empty_like(w, dtype=torch.int32)
     if T:
-        _call(_native_lib().moe_route_experts, index, logits.data_ptr(), _DTYPE[logits.dtype], logits.stride(0),
-              bias_ptr, T, E, top_k, _SCORE[score], n_group, topk_group, _GROUP_SCORE[group_score],
-              1 if renormalize else 0, scale, idx.data_ptr(), w.data_ptr())
+        _call(_native_lib().moe_route_experts, index,
+              _ROUTE(logits.data_ptr(), bias_ptr, idx.data_ptr(), w.data_ptr(), _current_stream(index), logits.stride(0),
+                     _DTYPE[logits.dtype], T, E, top_k, _SCORE[score], n_group, topk_group, _GROUP_SCORE[group_score],
+                     bool(renormalize), scale))
     return idx, w
 
 
@@ -137,9 +146,10 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, idx
         _fail("grad_weights must be a contiguous float32 [T, top_k] tensor on the logits' device")
     grad = logits.new_empty((T, E))
     if T:
-        _call(_native_lib().moe_route_experts_backward, index, grad_weights.data_ptr(), logits.data_ptr(),
-              _DTYPE[logits.dtype], logits.stride(0), idx.data_ptr(), T, E, idx.shape[1], _SCORE[score],
-              1 if renormalize else 0, scale, grad.data_ptr())
+        _call(_native_lib().moe_route_experts_backward, index,
+              _ROUTE_BACKWARD(grad_weights.data_ptr(), logits.data_ptr(), idx.data_ptr(), grad.data_ptr(),
+                              _current_stream(index), logits.stride(0), _DTYPE[logits.dtype], T, E, idx.shape[1],
+                              _SCORE[score], bool(renormalize), scale))
     return grad
 
 
@@ -215,9 +225,11 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: t
         _fail("out must be a contiguous [M, N] tensor of x's type on its device")
     if M:
         need = _linear_w4_workspace_bytes(M, N, K)
-        ws = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
-        _call(_native_lib().moe_linear_w4, index, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), codes.data_ptr(),
-              scale.data_ptr(), None if zero is None else zero.data_ptr(), group, M, N, K, out.data_ptr(), ws, need)
+        workspace = x.new_empty(need, dtype=torch.uint8) if need else None
+        _call(_native_lib().moe_linear_w4, index,
+              _LINEAR(x.data_ptr(), codes.data_ptr(), scale.data_ptr(), 0 if zero is None else zero.data_ptr(),
+                      out.data_ptr(), 0 if workspace is None else workspace.data_ptr(), _current_stream(index),
+                      x.stride(0), need, _DTYPE[x.dtype], group, M, N, K))
     return out
 
 
@@ -272,8 +284,10 @@ def experts_w4(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w13: t
     elif not (workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need
               and workspace.is_cuda and workspace.get_device() == index):
         _fail(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on x's device")
-    _call(_native_lib().moe_experts_w4, index, x.data_ptr(), _DTYPE[x.dtype], x.stride(0), idx.data_ptr(),
-          weights.data_ptr(), w13.data_ptr(), w13_scale.data_ptr(), None if w13_zero is None else w13_zero.data_ptr(),
-          w2.data_ptr(), w2_scale.data_ptr(), None if w2_zero is None else w2_zero.data_ptr(), group, T, top_k, E,
-          local_offset, H, I, out.data_ptr(), workspace.data_ptr(), workspace.numel())
+    _call(_native_lib().moe_experts_w4, index,
+          _EXPERTS(x.data_ptr(), idx.data_ptr(), weights.data_ptr(), w13.data_ptr(), w13_scale.data_ptr(),
+                   0 if w13_zero is None else w13_zero.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
+                   0 if w2_zero is None else w2_zero.data_ptr(), out.data_ptr(), workspace.data_ptr(),
+                   _current_stream(index), x.stride(0), workspace.numel(), _DTYPE[x.dtype], group, T, top_k, E,
+                   local_offset, H, I))
     return out

@@ -199,7 +199,8 @@ int moe_gate_quantize(const void* hidden_bf16, const void* gate_packed, int T, f
                       void* out_e4m3, float* out_scale, void* stream);
 
 /* ---- Expert router of any size and rule, its gradient, products with 4-bit weights ----
- * No reference counterparts: the reference has one fixed router and FP8 experts. Element types: */
+ * No reference counterparts: the reference has one fixed router and FP8 experts. Arguments come in a struct (they are
+ * many); pointers are device memory, the stream a cudaStream_t. Element types: */
 #define MOE_F32 0
 #define MOE_BF16 1
 #define MOE_F16 2
@@ -214,36 +215,63 @@ int moe_gate_quantize(const void* hidden_bf16, const void* gate_packed, int T, f
  *   renormalize  != 0: the weights are divided by their sum + 1e-20; then multiplied by `scale`
  * A logit or bias of -inf excludes an expert; where none is left idx is -1 and the weight 0. NaN logits give NaN
  * weights. 1 <= E <= 1024, top_k <= 32, n_group <= 32. Any alignment. */
-int moe_route_experts(const void* logits, int dtype, long long row_stride, const float* bias, int T, int E, int top_k,
-                      int score, int n_group, int topk_group, int group_score, int renormalize, float scale, int* idx,
-                      float* w, void* stream);
+typedef struct {
+  const void* logits;
+  const float* bias;
+  int* idx;
+  float* w;
+  void* stream;
+  long long row_stride;
+  int dtype, T, E, top_k, score, n_group, topk_group, group_score, renormalize;
+  float scale;
+} moe_route_experts_args;
+int moe_route_experts(const moe_route_experts_args* args);
 
 /* Gradient of moe_route_experts' weights: grad_w fp32 [T, top_k], the forward call's logits and idx (distinct
  * per row; values outside [0, E) take no part) -> grad_logits [T, E] contiguous, of the logits' type. */
-int moe_route_experts_backward(const float* grad_w, const void* logits, int dtype, long long row_stride, const int* idx,
-                               int T, int E, int top_k, int score, int renormalize, float scale, void* grad_logits,
-                               void* stream);
+typedef struct {
+  const float* grad_w;
+  const void* logits;
+  const int* idx;
+  void* grad_logits;
+  void* stream;
+  long long row_stride;
+  int dtype, T, E, top_k, score, renormalize;
+  float scale;
+} moe_route_experts_backward_args;
+int moe_route_experts_backward(const moe_route_experts_backward_args* args);
 
 /* 4-bit weights of a matrix [N, K]: codes [N, ceil(K / 2)] bytes, the even column in the low nibble; scale
  * [N, ceil(K / group)] of the activations' type (MOE_BF16 or MOE_F16); zero uint8 of the same shape (low four
  * bits), or NULL for 8; group 32, 64 or 128. Weight = scale * (code - zero). Stacked matrices follow one another.
  *
- * moe_linear_w4: out [M, N] = x . W^T, x [M, K] with rows x_stride elements apart, out contiguous, M up to 65535; both of type
- * `dtype`. Sums in fp32, rounded once. The workspace (256-byte aligned) is needed above 8 tokens; below, its size is 0
+ * moe_linear_w4: out [M, N] = x . W^T, x [M, K] with rows x_stride elements apart, out contiguous, M up to 65535 and x below 2^31 elements; both of type
+ * `dtype`. Sums in fp32, rounded once. The workspace (256-byte aligned) is needed above 16 tokens; below, its size is 0
  * and it may be NULL. */
 size_t moe_linear_w4_workspace_bytes(int M, int N, int K);
-int moe_linear_w4(const void* x, int dtype, long long x_stride, const void* codes, const void* scale, const void* zero,
-                  int group, int M, int N, int K, void* out, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct {
+  const void *x, *codes, *scale, *zero;
+  void *out, *workspace, *stream;
+  long long x_stride, workspace_bytes;
+  int dtype, group, M, N, K;
+} moe_linear_w4_args;
+int moe_linear_w4(const moe_linear_w4_args* args);
 
 /* Routed experts with 4-bit weights: for every token t and pick j whose expert e = idx[t, j] - local_offset is in
  * [0, E): out[t] += w[t, j] * W2[e] (X1 * silu(X2)), [X1 | X2] = W13[e] x[t]. x [T, H] with rows x_stride
  * elements apart; idx int32 and w fp32 [T, top_k]; w13 stacked [E, 2 I, H], w2 stacked [E, H, I]; out [T, H]
  * contiguous, of x's type (zeros for a token without a pick here). w13 and w2 16-byte, the workspace 256-byte aligned. 0 <= T <= 65535, top_k <= 32, E <= 1024. */
 size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I);
-int moe_experts_w4(const void* x, int dtype, long long x_stride, const int* idx, const float* w, const void* w13,
-                   const void* w13_scale, const void* w13_zero, const void* w2, const void* w2_scale,
-                   const void* w2_zero, int group, int T, int top_k, int E, int local_offset, int H, int I, void* out,
-                   void* workspace, size_t workspace_bytes, void* stream);
+typedef struct {
+  const void* x;
+  const int* idx;
+  const float* w;
+  const void *w13, *w13_scale, *w13_zero, *w2, *w2_scale, *w2_zero;
+  void *out, *workspace, *stream;
+  long long x_stride, workspace_bytes;
+  int dtype, group, T, top_k, E, local_offset, H, I;
+} moe_experts_w4_args;
+int moe_experts_w4(const moe_experts_w4_args* args);
 
 /* ---- Seeded synthetic inputs on the GPU (bit-identical to the CPU generator) ----
  * table: device fp32 [65537] inverse-normal-CDF table (see the Python package).

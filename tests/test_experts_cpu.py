@@ -22,36 +22,42 @@ def ptr():
 
 def test_router_refuses(lib, ptr):
     p = ptr[0]
+    ex = importlib.import_module("15642_moe_b200.experts")
     call = lambda dtype=0, T=4, E=64, k=4, score=0, ng=1, tg=1, gs=0, lg=p: lib.moe_route_experts(  # noqa: E731
-        lg, dtype, 64, None, T, E, k, score, ng, tg, gs, 1, 1.0, p, p, None)
+        ex._ROUTE(lg, 0, p, p, 0, 64, dtype, T, E, k, score, ng, tg, gs, 1, 1.0))
     for kw, word in [(dict(dtype=3), b"dtype"), (dict(T=-1), b"[T, E]"), (dict(E=0), b"[T, E]"), (dict(E=1025), b"[T, E]"),
                      (dict(k=0), b"top_k"), (dict(k=33), b"top_k"), (dict(k=9, ng=8), b"top_k"), (dict(ng=3), b"n_group"),
                      (dict(ng=64), b"n_group"), (dict(ng=4, tg=5), b"topk_group"), (dict(score=2), b"score"),
-                     (dict(E=32, ng=32, tg=8, gs=1), b"two"), (dict(lg=None), b"null")]:
+                     (dict(E=32, ng=32, tg=8, gs=1), b"two"), (dict(lg=0), b"null")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
-    assert call(T=0, lg=None) == 0
+    assert call(T=0, lg=0) == 0
+    assert lib.moe_route_experts(None) == 1 and b"null" in lib.moe_last_error()
     back = lambda dtype=0, T=4, E=64, k=4, score=0, g=p: lib.moe_route_experts_backward(  # noqa: E731
-        g, p, dtype, 64, p, T, E, k, score, 1, 1.0, p, None)
+        ex._ROUTE_BACKWARD(g, p, p, p, 0, 64, dtype, T, E, k, score, 1, 1.0))
     for kw, word in [(dict(dtype=-1), b"dtype"), (dict(E=0), b"[T, E]"), (dict(k=33), b"top_k"), (dict(score=5), b"score"),
-                     (dict(g=None), b"null")]:
+                     (dict(g=0), b"null")]:
         assert back(**kw) == 1 and word in lib.moe_last_error(), kw
     assert back(T=0) == 0
+    assert lib.moe_route_experts_backward(None) == 1
 
 
 def test_products_refuse(lib, ptr):
     p = ptr[0]
+    ex = importlib.import_module("15642_moe_b200.experts")
     call = lambda dtype=1, group=128, M=2, N=8, K=64, x=p: lib.moe_linear_w4(  # noqa: E731
-        x, dtype, 64, p, p, None, group, M, N, K, p, None, 0, None)
-    for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=16), b"group"), (dict(M=-1), b"[M, K]"), (dict(M=65536), b"65535"), (dict(N=0), b"[M, K]"),
-                     (dict(K=0), b"[M, K]"), (dict(x=None), b"null")]:
+        ex._LINEAR(x, p, p, 0, p, 0, 0, 64, 0, dtype, group, M, N, K))
+    for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=16), b"group"), (dict(M=-1), b"[M, K]"), (dict(M=65536), b"65535"),
+                     (dict(M=60000, K=70000), b"2^31"), (dict(N=0), b"[M, K]"), (dict(K=0), b"[M, K]"), (dict(x=0), b"null")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
     assert call(M=0) == 0
-    assert call(M=9) == 3 and b"workspace too small" in lib.moe_last_error()
-    assert lib.moe_linear_w4_workspace_bytes(8, 64, 64) == 0 and lib.moe_linear_w4_workspace_bytes(9, 64, 64) > 0
-    call = lambda dtype=1, group=128, T=2, k=2, E=4, H=64, I=32, ws=p, n=0, x=p: lib.moe_experts_w4(  # noqa: E731
-        x, dtype, 64, p, p, p, p, None, p, p, None, group, T, k, E, 0, H, I, p, ws, n, None)
+    assert call(M=17) == 3 and b"workspace too small" in lib.moe_last_error()
+    assert lib.moe_linear_w4_workspace_bytes(16, 64, 64) == 0 and lib.moe_linear_w4_workspace_bytes(17, 64, 64) > 0
+    assert lib.moe_linear_w4(None) == 1 and b"null" in lib.moe_last_error()
+    call = lambda dtype=1, group=128, T=2, k=2, E=4, H=64, I=32, ws=p, n=0, x=p, w2=p: lib.moe_experts_w4(  # noqa: E731
+        ex._EXPERTS(x, p, p, p, p, 0, w2, p, 0, p, ws, 0, 64, n, dtype, group, T, k, E, 0, H, I))
     for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=1), b"group"), (dict(T=65536), b"65535"), (dict(k=0), b"top_k"),
-                     (dict(E=1025), b"E must"), (dict(H=0), b"H and I"), (dict(x=None), b"null"), (dict(ws=None), b"null")]:
+                     (dict(E=1025), b"E must"), (dict(H=0), b"H and I"), (dict(x=0), b"null"), (dict(ws=0), b"null"),
+                     (dict(w2=p + 8), b"16-byte")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
     assert call(n=16) == 3 and b"workspace too small" in lib.moe_last_error()
     assert call(T=0) == 0
@@ -59,6 +65,30 @@ def test_products_refuse(lib, ptr):
     assert need > 0 and lib.moe_experts_w4_workspace_bytes(65535, 32, 256, 7168, 2048) > need
     assert lib.moe_experts_w4_workspace_bytes(65536, 2, 4, 64, 32) == 0
     assert call(ws=p + 16, n=1 << 40) == 1 and b"256-byte aligned" in lib.moe_last_error()
+    assert lib.moe_experts_w4(None) == 1
+
+
+def test_packed_arguments_have_the_structs_layout():
+    """Sizes of the packed arguments against the header's structs, compiled by a C compiler."""
+    import os
+    import struct
+    import subprocess
+    import tempfile
+    ex = importlib.import_module("15642_moe_b200.experts")
+    names = ["moe_route_experts_args", "moe_route_experts_backward_args", "moe_linear_w4_args", "moe_experts_w4_args"]
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with tempfile.TemporaryDirectory() as d:
+        src, exe = os.path.join(d, "a.c"), os.path.join(d, "a")
+        with open(src, "w") as f:
+            f.write('#include <stdio.h>\n#include <stddef.h>\n#include "moe_b200.h"\nint main(void) {\n'
+                    + "".join('printf("%%zu ", sizeof(%s));\n' % n for n in names)
+                    + 'printf("%zu %zu %zu %zu", offsetof(moe_route_experts_args, scale), offsetof(moe_route_experts_backward_args, scale),'
+                      ' offsetof(moe_linear_w4_args, K), offsetof(moe_experts_w4_args, I));\nreturn 0; }\n')
+        subprocess.run(["gcc", "-I", os.path.join(repo, "include"), "-o", exe, src], check=True)
+        got = [int(v) for v in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
+    packs = [ex._ROUTE.__self__, ex._ROUTE_BACKWARD.__self__, ex._LINEAR.__self__, ex._EXPERTS.__self__]
+    for size, at, pack in zip(got[:4], got[4:], packs):
+        assert pack.size - struct.calcsize("i") == at and pack.size <= size <= pack.size + 4   # the struct's own padding
 
 
 def test_python_layer_refuses_cpu_tensors(pkg):

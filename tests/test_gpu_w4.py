@@ -272,9 +272,9 @@ def test_refusals(pkg):
                          (dict(out=torch.zeros((3, 63), dtype=dtype, device="cuda")), "out")]:
         with pytest.raises((RuntimeError, TypeError), match=word):
             pkg.experts_w4(**{**ok, **change})
-    native = importlib.import_module("15642_moe_b200._native")
+    native, ex = (importlib.import_module("15642_moe_b200." + n) for n in ("_native", "experts"))
     ws = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
-    rc = native.cuda_lib().moe_experts_w4(x.data_ptr(), 1, 64, idx.data_ptr(), wt.data_ptr(), w13.data_ptr(), s13.data_ptr(), None,
-                                          w2.data_ptr(), s2.data_ptr(), None, 32, 3, 2, 3, 0, 64, 32, x.data_ptr(),
-                                          ws.data_ptr() + 16, 1 << 19, None)
+    rc = native.cuda_lib().moe_experts_w4(ex._EXPERTS(
+        x.data_ptr(), idx.data_ptr(), wt.data_ptr(), w13.data_ptr(), s13.data_ptr(), 0, w2.data_ptr(), s2.data_ptr(), 0, x.data_ptr(),
+        ws.data_ptr() + 16, 0, 64, 1 << 19, 1, 32, 3, 2, 3, 0, 64, 32))
     assert rc == 1 and b"256-byte aligned" in native.cuda_lib().moe_last_error()
