@@ -845,7 +845,7 @@ int w4_tma_codes(DeviceInfo* d, const uint8_t* codes, long long rows, int K, uin
 template <typename T>
 int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Matrix& w, int M, int N, int K, void* out, void* workspace,
                    cudaStream_t st) {
-  if (M <= WS_MAX_TOK) {
+  if (M <= WS_TOK) {
     const StreamArgs a{x, x_stride, w, M, N, K, out};
     return cuda_check(launch_w4_stream<T>(a, st), "linear_w4 launch");
   }
@@ -971,7 +971,7 @@ int moe_route_experts_backward(const moe_route_experts_backward_args* args) {
 }
 
 size_t moe_linear_w4_workspace_bytes(int M, int N, int K) {
-  if (M <= WS_MAX_TOK || N < 1 || K < 1) return 0;
+  if (M <= WS_TOK || N < 1 || K < 1) return 0;
   return make_linear_w4_ws(M, N, K).total;
 }
 
@@ -987,7 +987,7 @@ int moe_linear_w4(const moe_linear_w4_args* args) {
   if (!x || !codes || !scale || !out) return fail(MOE_ERR_INVALID, "moe_linear_w4: null pointer argument");
   const W4Matrix w{static_cast<const uint8_t*>(codes), scale, static_cast<const uint8_t*>(zero), group};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M > WS_MAX_TOK) {
+  if (M > WS_TOK) {
     const size_t need = moe_linear_w4_workspace_bytes(M, N, K);
     if (workspace == nullptr || workspace_bytes < need)
       return fail(MOE_ERR_WORKSPACE, "moe_linear_w4: workspace too small: need " + std::to_string(need) + " bytes");

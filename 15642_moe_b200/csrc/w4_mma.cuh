@@ -39,7 +39,8 @@ struct WmShape {
   static constexpr int D_COLS = NT * TERMS * (WM_STEP / G) >= 128 ? 128 : NT * TERMS * (WM_STEP / G);
   static constexpr int A_COL = 2 * D_COLS;
   static constexpr int A_SLOTS = (512 - A_COL) / 128;
-  // Warpgroups that scale, each TOK tokens of the tile: above 32 tokens one would be the slowest of the roles.
+  // Warpgroups that scale, each TOK tokens of the tile: above 32 tokens one would be the slowest of the roles (four for 128
+  // tokens took 8% longer than two: more warps on the same barriers).
   static constexpr int EPI = NT == 32 ? 1 : 2;
   static constexpr int TOK = NT / EPI;
   static constexpr int THREADS = 128 * (3 + EPI);
@@ -98,8 +99,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -167,6 +167,8 @@ __device__ __forceinline__ void fma16_scaled(float* acc, const float (&v)[16], f
 // Bounded wait of a converged warp, every lane for itself (each needs its own acquire); they agree on giving up. The
 // hardware suspends the lanes meanwhile: polling warps take issue slots and shared-memory cycles from the others.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int who) {
+  // A completed phase is seen by the plain test in a third of the suspending test's time.
+  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, who));
 }
 
@@ -287,7 +289,9 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
   }
-  if (MODE != WS_LINEAR) wait_prerequisite_grids();   // counts and rows come from the kernels before
+  // Counts come from the kernel before the first product; the second product may read them at once, since the first one
+  // lets it start only after its own wait, and load weights while the first still runs.
+  if (MODE == WS_UP) wait_prerequisite_grids();
   if (warp == 2) {
     if constexpr (MODE == WS_LINEAR) {
       if (lane == 0) {
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
           mbar_wait_drain(&ctl->c_full[(it - i) % S::CODE_STAGES], ((it - i) / S::CODE_STAGES) & 1u);
     } else if (warp == 2 && elect_one()) {
       // ---------------- token rows ----------------
-      if (MODE == WS_LINEAR) wait_prerequisite_grids();
+      if (MODE != WS_UP) wait_prerequisite_grids();          // rows come from the kernel before
       const uint64_t pol = policy_evict_last();
       uint32_t it = 0;
       for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
       int s = s0 + static_cast<int>((it ^ wg) & 1u);                   // the warpgroups take turns across units
       for (it += (it ^ wg) & 1u; it < end; it += 2, s += 2) {
         const uint32_t st = it % S::CODE_STAGES, slot = it % S::A_SLOTS;
-        uint32_t off[GPS];
+        W4Offset<W> off[GPS];
 #pragma unroll
         for (int i = 0; i < GPS; ++i) off[i] = w4_offset<W>(zrow ? __ldg(zrow + min(s * GPS + i, groups - 1)) & 15 : 8);
         if (!wait_warp(&ctl->c_full[st], (it / S::CODE_STAGES) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE) ||
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const uint4 x = *reinterpret_cast<const uint4*>(src + (((hf * 2 + c) ^ (srow & 7)) << 4));
-            const uint32_t o = off[(hf * 64 + c * 32) / G];
+            const W4Offset<W> o = off[(hf * 64 + c * 32) / G];
             const uint32_t word[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -600,7 +604,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
       }
     }
   }
-  if (MODE == WS_LINEAR) wait_prerequisite_grids();       // this grid ends after the one before it
+  if (MODE != WS_UP) wait_prerequisite_grids();           // this grid ends after the one before it
   __syncwarp();
   tc_fence_before();
   __syncthreads();

@@ -1,8 +1,8 @@
 /*
- * linear_w4 for up to 16 tokens, in one launch: the weights are read once, straight from global memory into matrix
+ * linear_w4 for up to 8 tokens, in one launch: the weights are read once, straight from global memory into matrix
  * fragments.
  *
- *   mma m16n8k16: A = 16 weight rows x 16 columns, B = 16 columns x 8 tokens, fp32 accumulators; one or two B per A.
+ *   mma m16n8k16: A = 16 weight rows x 16 columns, B = 16 columns x 8 tokens, fp32 accumulators.
  *
  * A thread holds, of rows g and g + 8 of a tile, the codes at a few places; which columns those are is free as long as A
  * and B agree. Thread t of a row's four takes group / 4 neighbouring columns of each group (one 16-, 8- or 4-byte load); a
@@ -25,7 +25,6 @@ namespace moe {
 constexpr int WS_WARPS = 8, WS_THREADS = 32 * WS_WARPS;
 constexpr int WS_ROWS = 16;                     // weight rows per block
 constexpr int WS_TOK = 8;                       // tokens per mma
-constexpr int WS_MAX_TOK = 16;                  // tokens that this kernel takes: two mma per fragment of weights
 constexpr int WS_STEP = 128;                    // columns per step
 
 enum { WS_LINEAR = 0, WS_UP = 1, WS_DOWN = 2 };  // which product a kernel computes: linear_w4, the experts' first, second
@@ -34,7 +33,7 @@ struct StreamArgs {
   const void* x;           // [M, K]
   long long x_stride;
   W4Matrix w;
-  int M, N, K;             // tokens (<= 16), output columns, reduction length
+  int M, N, K;             // tokens (<= 8), output columns, reduction length
   void* out;               // [M, N]
 };
 
@@ -54,25 +53,38 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Pair i of a word's codes (columns i and i + 4) as two numbers minus `off` (128 + zero or 1024 + zero, twice).
+// What a code's number is minus: 128 + zero twice in bf16; 1024 + zero and 64 + zero twice in f16 (all exact: zero < 16).
 template <typename T>
-__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int i, uint32_t off) {
-  constexpr bool F16 = std::is_same_v<T, __half>;
+struct W4Offset {
+  uint32_t a, b;
+};
+template <typename T>
+__device__ __forceinline__ W4Offset<T> w4_offset(int zero) {
+  const uint32_t z = static_cast<uint32_t>(zero);
+  if constexpr (std::is_same_v<T, __half>)
+    return {(0x6400u + z) * 0x10001u, (0x5400u + (z << 4)) * 0x10001u};
+  else
+    return {(0x4300u + z) * 0x10001u, 0u};
+}
+
+// Pair i of a word's codes (columns i and i + 4) as two numbers code - zero. A nibble in bits 0-3 of the mantissa of 128
+// (bf16) or 1024 (f16) adds its value; f16's ten bits also take one in bits 4-7, of 64, which saves two of three shifts.
+template <typename T>
+__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int i, const W4Offset<T>& off) {
   uint32_t v;
-  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(v) : "r"(word >> (4 * i)), "n"(F16 ? 0x64006400 : 0x43004300));
-  if constexpr (F16) {
-    const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&v), *reinterpret_cast<const __half2*>(&off));
+  if constexpr (std::is_same_v<T, __half>) {
+    const uint32_t w = i < 2 ? word : word >> 8;
+    if (i % 2 == 0)
+      asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(v) : "r"(w));
+    else
+      asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(v) : "r"(w));
+    const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&v), *reinterpret_cast<const __half2*>(i % 2 == 0 ? &off.a : &off.b));
     return *reinterpret_cast<const uint32_t*>(&d);
   } else {
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off));
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(v) : "r"(word >> (4 * i)));
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off.a));
     return *reinterpret_cast<const uint32_t*>(&d);
   }
-}
-// `off` for a zero point: both halves of 128 + z in bf16 (z < 16: exact) or 1024 + z in f16.
-template <typename T>
-__device__ __forceinline__ uint32_t w4_offset(int zero) {
-  const uint32_t one = (std::is_same_v<T, __half> ? 0x6400u : 0x4300u) + static_cast<uint32_t>(zero);
-  return one | (one << 16);
 }
 
 // 32 bits at any byte address; bytes at or past `left` are not read (only aligned words that hold a wanted byte).
@@ -158,13 +170,13 @@ __device__ __forceinline__ uint4 ld_x_pairs(const T* row, int k, int K, bool vec
   return make_uint4(pack2(e[0], e[4]), pack2(e[1], e[5]), pack2(e[2], e[6]), pack2(e[3], e[7]));
 }
 
-template <typename T, int G4, bool ALIGNED, int NB>
+template <typename T, int G4, bool ALIGNED>
 __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_constant__ StreamArgs p) {
   constexpr int GPS = 4 / G4;                    // groups per step
   // Steps in flight per warp, which is also how often the step's code is unrolled: the long ones (many groups, byte-wise
   // addresses) would spend more time fetching instructions than they win.
   constexpr int DEPTH = !ALIGNED ? 1 : G4 == 4 ? 4 : 2;
-  __shared__ float red[WS_WARPS][WS_ROWS][NB * WS_TOK];
+  __shared__ float red[WS_WARPS][WS_ROWS][WS_TOK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pitch = (p.K + 1) / 2, steps = (p.K + WS_STEP - 1) / WS_STEP;
   const int groups = (p.K + p.w.group - 1) / p.w.group;
@@ -174,13 +186,8 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
   const long long r0 = min(n0 + g, p.N - 1), r1 = min(n0 + g + 8, p.N - 1);   // rows past N repeat the last one
   const T *f0 = static_cast<const T*>(p.w.scale) + r0 * groups, *f1 = static_cast<const T*>(p.w.scale) + r1 * groups;
   const uint8_t *z0 = p.w.zero ? p.w.zero + r0 * groups : nullptr, *z1 = p.w.zero ? p.w.zero + r1 * groups : nullptr;
-  const T* xrow[NB];
-  bool vec = true;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    xrow[b] = static_cast<const T*>(p.x) + min(b * WS_TOK + g, p.M - 1) * p.x_stride;
-    vec = vec && (reinterpret_cast<uintptr_t>(xrow[b]) & 15u) == 0;
-  }
+  const T* xrow = static_cast<const T*>(p.x) + min(g, p.M - 1) * p.x_stride;
+  const bool vec = __all_sync(0xffffffffu, (reinterpret_cast<uintptr_t>(xrow) & 15u) == 0);
 
   // Steps that lie wholly inside the rows are read without a check per load (all of them where K is a multiple of 128 and
   // the rows allow 16-byte loads).
@@ -202,32 +209,29 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
   for (int d = 0; d < DEPTH; ++d)
     if (d < n) codes(a + d, buf[d]);
   // One step ahead: activations, scales and zero points.
-  uint4 x[NB][4];
+  uint4 x[4];
   float s0[GPS], s1[GPS];
-  uint32_t o0[GPS], o1[GPS];
+  W4Offset<T> o0[GPS], o1[GPS];
 #pragma unroll
-  for (int i = 0; i < 4 * NB; ++i) x[i / 4][i % 4] = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < 4; ++i) x[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int i = 0; i < GPS; ++i) o0[i] = o1[i] = w4_offset<T>(8);
   auto side = [&](int step) {
     const int k0 = step * WS_STEP;
+    if (g < p.M) {
+      if (step < whole) {
+        const T* xt = xrow + k0 + 8 * G4 * t;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (b * WS_TOK + g < p.M) {
-        if (step < whole) {
-          const T* xt = xrow[b] + k0 + 8 * G4 * t;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(xt + (i / G4) * (32 * G4) + (i % G4) * 8));
-            x[b][i] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                                 __byte_perm(v.y, v.w, 0x7632));
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[b][i] = ld_x_pairs<T>(xrow[b], k0 + (i / G4) * (32 * G4) + t * (8 * G4) + (i % G4) * 8, p.K, vec);
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(xt + (i / G4) * (32 * G4) + (i % G4) * 8));
+          x[i] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                            __byte_perm(v.y, v.w, 0x7632));
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ld_x_pairs<T>(xrow, k0 + (i / G4) * (32 * G4) + t * (8 * G4) + (i % G4) * 8, p.K, vec);
       }
+    }
 #pragma unroll
     for (int i = 0; i < GPS; ++i) {
       const int q = step < whole ? step * GPS + i : min(step * GPS + i, groups - 1);
@@ -239,9 +243,7 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
       }
     }
   };
-  float total[NB][4];
-#pragma unroll
-  for (int i = 0; i < 4 * NB; ++i) total[i / 4][i % 4] = 0.0f;
+  float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (n > 0) side(a);
   for (int s = 0; s < n; s += DEPTH) {
 #pragma unroll
@@ -250,11 +252,9 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
         const uint32_t u0[4] = {buf[d][0].x, buf[d][0].y, buf[d][0].z, buf[d][0].w};
         const uint32_t u1[4] = {buf[d][1].x, buf[d][1].y, buf[d][1].z, buf[d][1].w};
         if (s + d + DEPTH < n) codes(a + s + d + DEPTH, buf[d]);
-        uint4 xs[NB][4];
-#pragma unroll
-        for (int i = 0; i < 4 * NB; ++i) xs[i / 4][i % 4] = x[i / 4][i % 4];
+        const uint4 xs[4] = {x[0], x[1], x[2], x[3]};
         float fa[GPS], fb[GPS];
-        uint32_t oa[GPS], ob[GPS];
+        W4Offset<T> oa[GPS], ob[GPS];
 #pragma unroll
         for (int i = 0; i < GPS; ++i) {
           fa[i] = s0[i];
@@ -265,35 +265,23 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
         if (s + d + 1 < n) side(a + s + d + 1);
 #pragma unroll
         for (int q = 0; q < GPS; ++q) {
-          float acc[NB][4];
-#pragma unroll
-          for (int i = 0; i < 4 * NB; ++i) acc[i / 4][i % 4] = 0.0f;
+          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int i = q * G4; i < (q + 1) * G4; ++i) {
-            const uint32_t p0 = w4_pair<T>(u0[i], 0, oa[q]), p1 = w4_pair<T>(u0[i], 1, oa[q]), q0 = w4_pair<T>(u1[i], 0, ob[q]),
-                           q1 = w4_pair<T>(u1[i], 1, ob[q]);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) mma16816<T>(acc[b], p0, q0, p1, q1, xs[b][i].x, xs[b][i].y);
-            const uint32_t p2 = w4_pair<T>(u0[i], 2, oa[q]), p3 = w4_pair<T>(u0[i], 3, oa[q]), q2 = w4_pair<T>(u1[i], 2, ob[q]),
-                           q3 = w4_pair<T>(u1[i], 3, ob[q]);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) mma16816<T>(acc[b], p2, q2, p3, q3, xs[b][i].z, xs[b][i].w);
+            mma16816<T>(acc, w4_pair<T>(u0[i], 0, oa[q]), w4_pair<T>(u1[i], 0, ob[q]), w4_pair<T>(u0[i], 1, oa[q]),
+                        w4_pair<T>(u1[i], 1, ob[q]), xs[i].x, xs[i].y);
+            mma16816<T>(acc, w4_pair<T>(u0[i], 2, oa[q]), w4_pair<T>(u1[i], 2, ob[q]), w4_pair<T>(u0[i], 3, oa[q]),
+                        w4_pair<T>(u1[i], 3, ob[q]), xs[i].z, xs[i].w);
           }
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            total[b][0] = fmaf(fa[q], acc[b][0], total[b][0]);
-            total[b][1] = fmaf(fa[q], acc[b][1], total[b][1]);
-            total[b][2] = fmaf(fb[q], acc[b][2], total[b][2]);
-            total[b][3] = fmaf(fb[q], acc[b][3], total[b][3]);
-          }
+          total[0] = fmaf(fa[q], acc[0], total[0]);
+          total[1] = fmaf(fa[q], acc[1], total[1]);
+          total[2] = fmaf(fb[q], acc[2], total[2]);
+          total[3] = fmaf(fb[q], acc[3], total[3]);
         }
       }
   }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    *reinterpret_cast<float2*>(&red[warp][g][b * WS_TOK + 2 * t]) = make_float2(total[b][0], total[b][1]);
-    *reinterpret_cast<float2*>(&red[warp][g + 8][b * WS_TOK + 2 * t]) = make_float2(total[b][2], total[b][3]);
-  }
+  *reinterpret_cast<float2*>(&red[warp][g][2 * t]) = make_float2(total[0], total[1]);
+  *reinterpret_cast<float2*>(&red[warp][g + 8][2 * t]) = make_float2(total[2], total[3]);
   __syncthreads();
   const int row = threadIdx.x % WS_ROWS, tok = threadIdx.x / WS_ROWS;
   if (tok < p.M && n0 + row < p.N) {
@@ -304,21 +292,17 @@ __global__ void __launch_bounds__(WS_THREADS, 2) w4_stream_kernel(const __grid_c
   }
 }
 
-template <typename T, int NB>
-inline cudaError_t launch_w4_stream_nb(const StreamArgs& a, cudaStream_t st) {
+template <typename T>
+inline cudaError_t launch_w4_stream(const StreamArgs& a, cudaStream_t st) {
   const bool aligned = ((a.K + 1) / 2) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.w.codes) & 15u) == 0;
   const unsigned grid = (static_cast<unsigned>(a.N) + WS_ROWS - 1) / WS_ROWS;
   auto go = [&](auto kernel) { kernel<<<grid, WS_THREADS, 0, st>>>(a); };
   switch (a.w.group) {
-    case 128: aligned ? go(w4_stream_kernel<T, 4, true, NB>) : go(w4_stream_kernel<T, 4, false, NB>); break;
-    case 64: aligned ? go(w4_stream_kernel<T, 2, true, NB>) : go(w4_stream_kernel<T, 2, false, NB>); break;
-    default: aligned ? go(w4_stream_kernel<T, 1, true, NB>) : go(w4_stream_kernel<T, 1, false, NB>); break;
+    case 128: aligned ? go(w4_stream_kernel<T, 4, true>) : go(w4_stream_kernel<T, 4, false>); break;
+    case 64: aligned ? go(w4_stream_kernel<T, 2, true>) : go(w4_stream_kernel<T, 2, false>); break;
+    default: aligned ? go(w4_stream_kernel<T, 1, true>) : go(w4_stream_kernel<T, 1, false>); break;
   }
   return cudaGetLastError();
-}
-template <typename T>
-inline cudaError_t launch_w4_stream(const StreamArgs& a, cudaStream_t st) {
-  return a.M <= WS_TOK ? launch_w4_stream_nb<T, 1>(a, st) : launch_w4_stream_nb<T, 2>(a, st);
 }
 
 }  // namespace moe

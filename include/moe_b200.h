@@ -246,7 +246,7 @@ int moe_route_experts_backward(const moe_route_experts_backward_args* args);
  * bits), or NULL for 8; group 32, 64 or 128. Weight = scale * (code - zero). Stacked matrices follow one another.
  *
  * moe_linear_w4: out [M, N] = x . W^T, x [M, K] with rows x_stride elements apart, out contiguous, M up to 65535 and x below 2^31 elements; both of type
- * `dtype`. Sums in fp32, rounded once. The workspace (256-byte aligned) is needed above 16 tokens; below, its size is 0
+ * `dtype`. Sums in fp32, rounded once. The workspace (256-byte aligned) is needed above 8 tokens; below, its size is 0
  * and it may be NULL. */
 size_t moe_linear_w4_workspace_bytes(int M, int N, int K);
 typedef struct {

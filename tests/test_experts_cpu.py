@@ -50,8 +50,8 @@ def test_products_refuse(lib, ptr):
                      (dict(M=60000, K=70000), b"2^31"), (dict(N=0), b"[M, K]"), (dict(K=0), b"[M, K]"), (dict(x=0), b"null")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
     assert call(M=0) == 0
-    assert call(M=17) == 3 and b"workspace too small" in lib.moe_last_error()
-    assert lib.moe_linear_w4_workspace_bytes(16, 64, 64) == 0 and lib.moe_linear_w4_workspace_bytes(17, 64, 64) > 0
+    assert call(M=9) == 3 and b"workspace too small" in lib.moe_last_error()
+    assert lib.moe_linear_w4_workspace_bytes(8, 64, 64) == 0 and lib.moe_linear_w4_workspace_bytes(9, 64, 64) > 0
     assert lib.moe_linear_w4(None) == 1 and b"null" in lib.moe_last_error()
     call = lambda dtype=1, group=128, T=2, k=2, E=4, H=64, I=32, ws=p, n=0, x=p, w2=p: lib.moe_experts_w4(  # noqa: E731
         ex._EXPERTS(x, p, p, p, p, 0, w2, p, 0, p, ws, 0, 64, n, dtype, group, T, k, E, 0, H, I))
