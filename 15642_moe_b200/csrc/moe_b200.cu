@@ -917,8 +917,11 @@ int experts_w4_impl(DeviceInfo* d, const ExpertsW4Args& p, void* out, uint8_t* W
   if (int rc = launch_w4_mma<T, WS_UP>(d, up, xg, routes, tile, st)) return rc;
   if (int rc = launch_w4_mma<T, WS_DOWN>(d, down, h, 2ll * routes, tile, st)) return rc;
   const int vec = p.H % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
-  return cuda_check(launch_programmatic_3d(experts_combine_kernel<T>, dim3((p.H + 1023) / 1024, p.T), 256, 0, st, static_cast<const float*>(y),
-                                           static_cast<const int*>(slot), p.wt, p.k, p.H, vec, static_cast<T*>(out)),
+  // Whole tokens per block once there are enough of them to fill the SMs twice; else 1024 columns.
+  const int span = p.T >= 2 * d->num_sms ? round_up(p.H, 1024) : 1024;
+  return cuda_check(launch_programmatic_3d(experts_combine_kernel<T>, dim3((p.H + span - 1) / span, p.T), 256, 0, st,
+                                           static_cast<const float*>(y), static_cast<const int*>(slot), p.wt, p.k, p.H, span, vec,
+                                           static_cast<T*>(out)),
                     "experts_combine launch");
 }
 

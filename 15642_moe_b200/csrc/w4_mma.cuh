@@ -379,7 +379,6 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
         const uint32_t idesc = (1u << 4) | fmt | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
         for (int s = s0; s < s1; ++s, ++a_it) {
           const uint32_t slot = a_it % S::A_SLOTS;
-          if (!mbar_wait_spin(&ctl->a_full[slot], (a_it / S::A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA)) goto mma_end;
           const uint32_t a = tmem + S::A_COL + slot * 128;
           uint64_t bd = b_desc0;
           uint32_t d = 0;
@@ -396,6 +395,8 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
                 if (!mbar_wait_spin(&ctl->d_empty[d_it & 1], ((d_it >> 1) & 1u) ^ 1u, abort_flag, ST_TIMEOUT_MMA)) goto mma_end;
                 d = tmem + (d_it & 1) * S::D_COLS;
               }
+              // The weights come last, as a rule: nothing else is waited for between them and the step's first mma.
+              if (k == 0 && !mbar_wait_spin(&ctl->a_full[slot], (a_it / S::A_SLOTS) & 1u, abort_flag, ST_TIMEOUT_MMA)) goto mma_end;
               if (k % (G * GPB) == 0 || c % BC == 0) tc_fence_after();
 #pragma unroll
               for (int kk = 0; kk < 4 / PARTS; ++kk) {
@@ -766,10 +767,11 @@ __global__ void __launch_bounds__(256) experts_gather_kernel(const T* x, long lo
   }
 }
 
-// out[t] = sum over the token's local picks, in their order, of weight * y[row], rounded once. Blocks of 1024 columns
-// of a token; `vec`: 4 neighbouring columns per thread (H a multiple of 4, out 8-byte aligned).
+// out[t] = sum over the token's local picks, in their order, of weight * y[row], rounded once. A block has `span` columns of
+// a token (a multiple of 1024). `vec`: 4 neighbouring columns per thread (H a multiple of 4, out 8-byte aligned).
 template <typename T>
-__global__ void __launch_bounds__(256) experts_combine_kernel(const float* y, const int* place, const float* wt, int k, int H, int vec, T* out) {
+__global__ void __launch_bounds__(256) experts_combine_kernel(const float* y, const int* place, const float* wt, int k, int H, int span, int vec,
+                                                              T* out) {
   __shared__ int row[RX_MAX_K];
   __shared__ float weight[RX_MAX_K];
   __shared__ int count;
@@ -787,22 +789,39 @@ __global__ void __launch_bounds__(256) experts_combine_kernel(const float* y, co
     if (lane == 0) count = __popc(m);
   }
   __syncthreads();
-  const int n = count, c = blockIdx.x * 1024 + threadIdx.x * (vec ? 4 : 1);
+  const int n = count, begin = blockIdx.x * span, end = min(H, begin + span);
   if (vec) {
-    if (c >= H) return;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int j = 0; j < n; ++j) {
-      const float4 v = __ldcs(reinterpret_cast<const float4*>(y + static_cast<long long>(row[j]) * H + c));
-      const float w = weight[j];
-      acc.x = fmaf(w, v.x, acc.x);
-      acc.y = fmaf(w, v.y, acc.y);
-      acc.z = fmaf(w, v.z, acc.z);
-      acc.w = fmaf(w, v.w, acc.w);
+    // Up to 4 pieces of 1024 columns at a time, their loads together in flight.
+    for (int c0 = begin; c0 < end; c0 += 4096) {
+      float4 acc[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int j = 0; j < n; ++j) {
+        const float* src = y + static_cast<long long>(row[j]) * H + c0 + threadIdx.x * 4;
+        const float w = weight[j];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c0 + i * 1024 + static_cast<int>(threadIdx.x) * 4 < end) v[i] = __ldcs(reinterpret_cast<const float4*>(src + i * 1024));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c0 + i * 1024 + static_cast<int>(threadIdx.x) * 4 < end) {
+            acc[i].x = fmaf(w, v[i].x, acc[i].x);
+            acc[i].y = fmaf(w, v[i].y, acc[i].y);
+            acc[i].z = fmaf(w, v[i].z, acc[i].z);
+            acc[i].w = fmaf(w, v[i].w, acc[i].w);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + i * 1024 + threadIdx.x * 4;
+        if (c < end)
+          *reinterpret_cast<uint2*>(out + t * H + c) =
+              make_uint2(pack2(from_f32<T>(acc[i].x), from_f32<T>(acc[i].y)), pack2(from_f32<T>(acc[i].z), from_f32<T>(acc[i].w)));
+      }
     }
-    *reinterpret_cast<uint2*>(out + t * H + c) =
-        make_uint2(pack2(from_f32<T>(acc.x), from_f32<T>(acc.y)), pack2(from_f32<T>(acc.z), from_f32<T>(acc.w)));
   } else {
-    for (int i = c; i < min(H, static_cast<int>(blockIdx.x + 1) * 1024); i += 256) {
+    for (int i = begin + threadIdx.x; i < end; i += 256) {
       float acc = 0.0f;
       for (int j = 0; j < n; ++j) acc = fmaf(weight[j], y[static_cast<long long>(row[j]) * H + i], acc);
       out[t * H + i] = from_f32<T>(acc);
