@@ -19,6 +19,11 @@
  *   3. each candidate counts the candidates before it; that rank is its place in the output.
  * More than 32 candidates (many equal scores, or the best ones side by side in a few lanes): k rounds of
  * arg-max over the warp instead, with the same result.
+ *
+ * Measured on a B200 (device time): 16384 tokens, 256 experts, sigmoid, bias, 8 groups, top 8: 13.2 us, 1.3 TB/s of
+ * logits; 3.8 us for 4096 tokens without groups and bias; one token 2.7 us. Bound by instructions (three
+ * quarters of the issue slots at 16384 tokens), not by memory: the floor there is 2.8 us. The first version,
+ * with accurate exponentials for the choice and one lane per group, took 34 us.
  */
 #pragma once
 #include "moe_common.cuh"
@@ -341,6 +346,9 @@ struct RouteExpertsBwdArgs {
  *   softmax: dl_e = s_e (ds_e - sum_i ds_i s_i). With renormalisation the sum is
  *            (sum g s / D) (1e-20 / D): the two terms that cancel are never formed.
  * The choice itself (idx) has no gradient, nor has the bias.
+ *
+ * A row is written twice where it was picked: first every expert's value without a pick, then the picks over it. That
+ * needs no shared memory (7.0 us either way at 16384 x 256, sigmoid; the floor is 2.8 us, most of it the dense output).
  */
 template <typename T, int VPT>
 __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_backward_kernel(const __grid_constant__ RouteExpertsBwdArgs p) {

@@ -13,6 +13,12 @@
  * Split: a block has one tile of 16 rows, its 8 warps an eighth of the columns each; their sums meet in shared memory in
  * warp order, so results repeat bit for bit. Nothing is staged: a warp alone uses its columns of x. 1 to 4 steps of 128
  * columns are in flight per warp (1 KB each).
+ *
+ * Measured on a B200 (device time, group 128): 4096 x 7168 for one token 8.5 us (1.8 TB/s of codes), for 8 tokens 10.1 us;
+ * 7168 x 2048 6.3 us; 28672 x 7168 47.7 us (2.2 TB/s). Bound by instructions: about 19 per 256 weights, of which the
+ * conversion has 11. An e4m3 mma would need no conversion (a code's byte is an e4m3 number), but mma.sync with it
+ * took some 30 issue slots on sm_100a, more than the conversion. Staging activations and scales in
+ * shared memory, with the columns split over a cluster, took 14 us for the first shape.
  */
 #pragma once
 #include "gate.cuh"
