@@ -31,6 +31,7 @@
 #include <cudaTypedefs.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <cstring>
 #include <mutex>
 #include <utility>
@@ -677,6 +678,23 @@ namespace {
 
 int round_up(long long v, int to) { return static_cast<int>((v + to - 1) / to * to); }
 int w4_bytes(int K) { return static_cast<int>((static_cast<long long>(K) + 1) / 2); }
+// Bytes from the first to the last element of `rows` rows of 16-bit elements.
+size_t row_bytes(int rows, long long stride, int columns) {
+  return (static_cast<size_t>(rows - 1) * static_cast<size_t>(stride < 0 ? 0 : stride) + columns) * 2;
+}
+struct Span {
+  const void* p;
+  size_t n;
+};
+// Blocks write output rows while others still read inputs, so the output may overlap none of them.
+bool overlaps(const void* out, size_t n, std::initializer_list<Span> in) {
+  const uintptr_t o0 = reinterpret_cast<uintptr_t>(out), o1 = o0 + n;
+  for (const Span& s : in) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(s.p);
+    if (s.n != 0 && a < o1 && o0 < a + s.n) return true;
+  }
+  return false;
+}
 // TMA wants rows that start on 16-byte boundaries.
 bool w4_rows_aligned(const void* codes, int K) { return w4_bytes(K) % 16 == 0 && aligned16(codes); }
 
@@ -859,6 +877,7 @@ int linear_w4_impl(DeviceInfo* d, const void* x, long long x_stride, const W4Mat
   linear_w4_layout_kernel<T><<<row_blocks + code_blocks, 256, 0, st>>>(static_cast<const T*>(x), x_stride, M, K, reinterpret_cast<T*>(W + ws.x),
                                                                       row_blocks, w.codes, N, W + ws.codes);
   if (copy) a.w.codes = W + ws.codes;
+  a.codes_copied = copy ? 1 : 0;
   a.E = 1;
   a.N = N;
   a.K = K;
@@ -997,6 +1016,10 @@ int moe_linear_w4(const moe_linear_w4_args* args) {
     if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
       return fail(MOE_ERR_INVALID, "moe_linear_w4: workspace must be 256-byte aligned");
   }
+  const size_t m = static_cast<size_t>(M), groups = (static_cast<size_t>(K) + group - 1) / group, n = static_cast<size_t>(N);
+  if (overlaps(out, m * n * 2, {{x, row_bytes(M, x_stride, K)}, {codes, n * w4_bytes(K)}, {scale, n * groups * 2}, {zero, zero ? n * groups : 0},
+                                {workspace, moe_linear_w4_workspace_bytes(M, N, K)}}))
+    return fail(MOE_ERR_INVALID, "moe_linear_w4: the output overlaps an input or the workspace");
   DeviceInfo* d = nullptr;
   if (int rc = device_info(&d)) return rc;
   return dtype == MOE_BF16 ? linear_w4_impl<__nv_bfloat16>(d, x, x_stride, w, M, N, K, out, workspace, st)
@@ -1020,6 +1043,7 @@ int moe_experts_w4(const moe_experts_w4_args* args) {
   if (static_cast<long long>(E) * (2ll * I > H ? 2ll * I : H) > 0x7FFFFFFFll)
     return fail(MOE_ERR_INVALID, "moe_experts_w4: the experts' matrices have more than 2^31 rows");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_experts_w4: group must be 32, 64 or 128");
+  if (local_offset < 0) return fail(MOE_ERR_INVALID, "moe_experts_w4: local_offset must not be negative");
   if (T == 0) return MOE_OK;
   if (!x || !idx || !w || !w13 || !w13_scale || !w2 || !w2_scale || !out || !workspace)
     return fail(MOE_ERR_INVALID, "moe_experts_w4: null pointer argument");
@@ -1029,6 +1053,15 @@ int moe_experts_w4(const moe_experts_w4_args* args) {
     return fail(MOE_ERR_WORKSPACE, "moe_experts_w4: workspace too small: need " + std::to_string(need) + " bytes");
   if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
     return fail(MOE_ERR_INVALID, "moe_experts_w4: workspace must be 256-byte aligned");
+  {
+    const size_t e = static_cast<size_t>(E), picks = static_cast<size_t>(T) * top_k, h = static_cast<size_t>(H), i = static_cast<size_t>(I);
+    const size_t g13 = (h + group - 1) / group, g2 = (i + group - 1) / group;
+    if (overlaps(out, static_cast<size_t>(T) * h * 2,
+                 {{x, row_bytes(T, x_stride, H)}, {idx, picks * 4}, {w, picks * 4}, {w13, e * 2 * i * w4_bytes(H)}, {w13_scale, e * 2 * i * g13 * 2},
+                  {w13_zero, w13_zero ? e * 2 * i * g13 : 0}, {w2, e * h * w4_bytes(I)}, {w2_scale, e * h * g2 * 2},
+                  {w2_zero, w2_zero ? e * h * g2 : 0}, {workspace, need}}))
+      return fail(MOE_ERR_INVALID, "moe_experts_w4: the output overlaps an input or the workspace");
+  }
   const ExpertsW4Args a{x, x_stride, idx, w,
                         {static_cast<const uint8_t*>(w13), w13_scale, static_cast<const uint8_t*>(w13_zero), group},
                         {static_cast<const uint8_t*>(w2), w2_scale, static_cast<const uint8_t*>(w2_zero), group},

@@ -87,6 +87,7 @@ struct WmArgs {
   W4Matrix w;
   int E, N, K;              // experts; output columns (up: I) and reduction length of one
   int M;                    // linear: tokens
+  int codes_copied;         // linear: the codes come from the kernel before, too
   const int* counts;        // [E] routes per expert (up, down)
   int row_cap;              // rows of the route-ordered buffers
   int splits, sps;          // linear: parts of the columns, each of `sps` steps
@@ -332,6 +333,10 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
     if constexpr (S::EPI == 2) regs_dec<WM_REGS_CTRL>();
     if (warp == 0 && elect_one()) {
       // ---------------- codes ----------------
+      if (MODE == WS_LINEAR && p.codes_copied) {
+        wait_prerequisite_grids();
+        fence_proxy_async_global();
+      }
       const uint64_t pol = policy_evict_first();
       uint32_t it = 0;
       for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
@@ -352,6 +357,7 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
     } else if (warp == 2 && elect_one()) {
       // ---------------- token rows ----------------
       if (MODE != WS_UP) wait_prerequisite_grids();          // rows come from the kernel before
+      fence_proxy_async_global();                           // its stores, then this thread's copies
       const uint64_t pol = policy_evict_last();
       uint32_t it = 0;
       for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {

@@ -164,6 +164,7 @@ class _RouteExperts(torch.autograd.Function):
         return idx, w
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, _, grad_weights):
         logits, idx = ctx.saved_tensors
         grad = route_experts_backward(grad_weights.contiguous(), logits, idx, **ctx.rule)
@@ -208,7 +209,7 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: t
     """x [M, K] (bfloat16 or float16, rows any distance apart) times the 4-bit W [N, K]: [M, N] in x's type.
 
     ``codes``, ``scale``, ``zero`` as in this module's description, ``group`` 32, 64 or 128. M up to 65535, any N and
-    K from 1 on. Sums are held in 32 bits and rounded once."""
+    K from 1 on. ``out`` may not overlap an input. Sums are held in 32 bits and rounded once."""
     _check_x(x, group, "[M, K]")
     if codes.dim() != 2:
         _fail("codes must be [N, ceil(K / 2)]")
@@ -251,8 +252,8 @@ def experts_w4(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w13: t
 
     ``x`` [T, H] bfloat16 or float16, rows any distance apart; ``idx`` int32 and ``weights`` fp32 [T, top_k], as
     route_experts returns them; ``w13`` codes uint8 [E, 2 I, ceil(H / 2)], ``w2`` codes uint8 [E, H, ceil(I / 2)]
-    (16-byte aligned), scales and zero points as in this module's description. T up to 65535. Sums are held in 32 bits
-    and rounded once."""
+    (16-byte aligned), scales and zero points as in this module's description. T up to 65535. ``out`` may not overlap an
+    input. Sums are held in 32 bits and rounded once."""
     _check_x(x, group, "[T, H]")
     if not (w13.dim() == 3 and w13.shape[1] % 2 == 0):
         _fail("w13 must be [E, 2 I, ceil(H / 2)]")

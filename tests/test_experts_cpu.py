@@ -44,20 +44,21 @@ def test_router_refuses(lib, ptr):
 def test_products_refuse(lib, ptr):
     p = ptr[0]
     ex = importlib.import_module("15642_moe_b200.experts")
-    call = lambda dtype=1, group=128, M=2, N=8, K=64, x=p: lib.moe_linear_w4(  # noqa: E731
-        ex._LINEAR(x, p, p, 0, p, 0, 0, 64, 0, dtype, group, M, N, K))
+    call = lambda dtype=1, group=128, M=2, N=8, K=64, x=p, out=p + 2048: lib.moe_linear_w4(  # noqa: E731
+        ex._LINEAR(x, p, p, 0, out, 0, 0, 64, 0, dtype, group, M, N, K))
     for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=16), b"group"), (dict(M=-1), b"[M, K]"), (dict(M=65536), b"65535"),
-                     (dict(M=60000, K=70000), b"2^31"), (dict(N=0), b"[M, K]"), (dict(K=0), b"[M, K]"), (dict(x=0), b"null")]:
+                     (dict(M=60000, K=70000), b"2^31"), (dict(N=0), b"[M, K]"), (dict(K=0), b"[M, K]"), (dict(x=0), b"null"),
+                     (dict(out=p + 64), b"overlaps")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
     assert call(M=0) == 0
     assert call(M=9) == 3 and b"workspace too small" in lib.moe_last_error()
     assert lib.moe_linear_w4_workspace_bytes(8, 64, 64) == 0 and lib.moe_linear_w4_workspace_bytes(9, 64, 64) > 0
     assert lib.moe_linear_w4(None) == 1 and b"null" in lib.moe_last_error()
-    call = lambda dtype=1, group=128, T=2, k=2, E=4, H=64, I=32, ws=p, n=0, x=p, w2=p: lib.moe_experts_w4(  # noqa: E731
-        ex._EXPERTS(x, p, p, p, p, 0, w2, p, 0, p, ws, 0, 64, n, dtype, group, T, k, E, 0, H, I))
+    call = lambda dtype=1, group=128, T=2, k=2, E=4, H=64, I=32, ws=p, n=0, x=p, w2=p, off=0: lib.moe_experts_w4(  # noqa: E731
+        ex._EXPERTS(x, p, p, p, p, 0, w2, p, 0, p, ws, 0, 64, n, dtype, group, T, k, E, off, H, I))
     for kw, word in [(dict(dtype=0), b"bf16"), (dict(group=1), b"group"), (dict(T=65536), b"65535"), (dict(k=0), b"top_k"),
                      (dict(E=1025), b"E must"), (dict(H=0), b"H and I"), (dict(x=0), b"null"), (dict(ws=0), b"null"),
-                     (dict(w2=p + 8), b"16-byte")]:
+                     (dict(w2=p + 8), b"16-byte"), (dict(off=-1), b"local_offset"), (dict(n=1 << 40), b"overlaps")]:
         assert call(**kw) == 1 and word in lib.moe_last_error(), kw
     assert call(n=16) == 3 and b"workspace too small" in lib.moe_last_error()
     assert call(T=0) == 0

@@ -120,6 +120,32 @@ def test_linear_repeats_bit_for_bit_and_captures(pkg):
         assert torch.equal(out, pkg.linear_w4(x, *w))
 
 
+@pytest.mark.parametrize("M", [20, 100])
+def test_alternating_weights_of_an_odd_width(pkg, M):
+    """Rows that TMA cannot read are copied within the call: every call has to see its own weights."""
+    dtype, N, K = torch.bfloat16, 3000, 1999
+    sets = [weights((), N, K, 64, True, dtype, seed) for seed in (1, 2, 3)]
+    x = torch.randn((M, K), generator=torch.Generator().manual_seed(M)).to(dtype).cuda()
+    first = [check_linear(pkg, x, *w, 64) for w in sets]
+    for i in range(30):
+        assert torch.equal(pkg.linear_w4(x, *sets[i % 3], group=64), first[i % 3])
+
+
+def test_overlapping_output_is_refused(pkg):
+    dtype = torch.bfloat16
+    w = weights((), 64, 64, 32, False, dtype, 1)
+    for M in (2, 40):
+        x = torch.zeros((M, 64), dtype=dtype, device="cuda")
+        with pytest.raises(RuntimeError, match="overlaps"):
+            pkg.linear_w4(x, *w, group=32, out=x)
+    l13, l2 = layer(2, 64, 32, 32, False, dtype, 0)
+    idx, wt = routing(40, 2, 1, 0)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        pkg.experts_w4(x, idx, wt, l13[0], l13[1], l2[0], l2[1], group=32, out=x)
+    with pytest.raises(RuntimeError, match="local_offset"):
+        pkg.experts_w4(x, idx, wt, l13[0], l13[1], l2[0], l2[1], group=32, local_offset=-1)
+
+
 def test_offsets_past_32_bits(pkg):
     """Codes of more than 2^32 bytes: the last rows of a very tall matrix."""
     N, K = 2 ** 20 + 77, 8192
