@@ -705,6 +705,8 @@ constexpr int WM_MAX_ROWS = 65535;   // rows of x: a grid dimension of the kerne
 constexpr int WM_SMS = 148;   // the split rule's SM count: results and workspace sizes do not depend on the device
 
 // linear_w4: parts of the columns, so that few row tiles still fill the SMs; two steps each at least.
+// Device us with at least two, three, six steps: 13 x 1001 x 1999 10.5, 12.1, 14.9; 64 x 2048 x 4096 12.2, 13.0, 14.5;
+// 16 x 2048 x 4096 10.2, 9.6, 11.2.
 int wm_splits(int M, int N, int K) {
   const long long nt = wm_tile(M), units = (M + nt - 1) / nt * ((N + 127ll) / 128);
   const int steps = (K + WM_STEP - 1) / WM_STEP;

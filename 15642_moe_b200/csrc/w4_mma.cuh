@@ -17,11 +17,13 @@
  * the units (token tile, 128 weight rows[, part of the columns]).
  *
  * Measured on a B200 (device time, 32 experts of 7168 x 2048, group 128): T = 64 of a 256-expert layer 188 us, 3.3 TB/s of
- * weights; T = 4096 740 us, 490 TFLOP/s; linear_w4 512 x 4096 x 7168 39 us, 770 TFLOP/s. What bounds it, by leaving parts
+ * weights; T = 4096 742 to 745 us, 485 TFLOP/s; linear_w4 512 x 4096 x 7168 39 us, 770 TFLOP/s. What bounds it, by leaving parts
  * out: T = 64 took 182 us whole, 159 without the conversion, 168 without the mma, 170 without the scaling, 143 without
- * conversion and its stores, which is what loading the weights and the waves of units take; the roles' latencies add the
- * rest. T = 4096 took 680 to 760 us whichever part was left out: a step brings 16 KB of codes and up to 64 KB of token rows
- * into the SM, which at about 64 bytes a cycle is as long as its mma. Pairs of SMs that share the token rows
+ * conversion and its stores, about what loading the weights and the waves of units take. Leaving out parts shifts the other
+ * roles' waits too (199 us without the stores alone), so these bound the shares and do not add up. T = 4096 took 749 us whole,
+ * 683 to 758 without one of the first three and 808 without the stores alone, so none of them alone is the limit. What is left
+ * is the way into the SM: a step brings 16 KB of codes and up to 64 KB of token rows, which at 64 bytes a cycle (reckoned,
+ * not measured by itself) is as long as its mma. Pairs of SMs that share the token rows
  * (cta_group::2) would halve that.
  */
 #pragma once

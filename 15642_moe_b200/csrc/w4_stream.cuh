@@ -14,8 +14,9 @@
  * warp order, so results repeat bit for bit. Nothing is staged: a warp alone uses its columns of x. 1 to 4 steps of 128
  * columns are in flight per warp (1 KB each).
  *
- * Measured on a B200 (device time, group 128): 4096 x 7168 for one token 8.5 us (1.8 TB/s of codes), for 8 tokens 10.1 us;
- * 7168 x 2048 6.3 us; 28672 x 7168 47.7 us (2.2 TB/s). Bound by instructions: about 19 per 256 weights, of which the
+ * Measured on a B200 (device time, group 128): 4096 x 7168 for one token 8.5 to 9.6 us, from one B200 to another (1.5 to
+ * 1.7 TB/s of codes; three copies of the weights in turn, which L2 holds), for 8 tokens 9.9 us; 7168 x 2048 6.2 us;
+ * 28672 x 7168, which L2 does not hold so, 47.8 us (2.1 TB/s), for 8 tokens 55.7 us. Bound by instructions: about 19 per 256 weights, of which the
  * conversion has 11. An e4m3 mma would need no conversion (a code's byte is an e4m3 number), but mma.sync with it
  * took some 30 issue slots on sm_100a, more than the conversion. Staging activations and scales in
  * shared memory, with the columns split over a cluster, took 14 us for the first shape.
