@@ -393,10 +393,12 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_backward_kernel(c
     d = __fdiv_rn(g - __fdiv_rn(gs, D), D);
     dot = __fdiv_rn(gs, D) * __fdiv_rn(1e-20f, D);
   }
-  // Every expert's value without a pick, then the picks over them.
+  // Every expert's value without a pick, then the picks over them. A row without a pick has constant weights: zeros, also
+  // where all its logits are -inf and the softmax is NaN.
+  const bool dense = p.softmax && __any_sync(0xffffffffu, e >= 0);
   float o[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) o[i] = p.softmax ? -(x[i] * inv) * dot : 0.0f;
+  for (int i = 0; i < VPT; ++i) o[i] = dense ? -(x[i] * inv) * dot : 0.0f;
   T* out = static_cast<T*>(p.grad_logits) + t * p.E;
   if (p.E == 32 * VPT && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
     constexpr int BYTES = VPT * static_cast<int>(sizeof(T)) < 16 ? VPT * static_cast<int>(sizeof(T)) : 16;

@@ -53,6 +53,8 @@ def route_grad(grad_w, logits, idx, score, renormalize, scale):
     out = np.zeros((T, E))
     for t in range(T):
         js = [j for j in range(idx.shape[1]) if 0 <= idx[t, j] < E]
+        if not js:                                   # constant weights, also where the softmax of the row is NaN
+            continue
         ds = np.zeros(E)
         D = sum(s[t, idx[t, j]] for j in js) + 1e-20
         for j in js:

@@ -1,0 +1,48 @@
+"""The general router at rows where it is easily wrong: no expert left, scores that round together, small differences.
+
+The gradient of a row without a pick is exactly zero: its weights are constants."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import experts_oracle as X
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("E", [1, 60, 64, 256, 1000])
+def test_gradient_of_a_row_without_experts(pkg, E, score, renormalize, dtype):
+    k = min(E, 6)
+    x = torch.randn((9, E), generator=torch.Generator().manual_seed(E)).to(dtype).cuda()
+    x[2] = x[8] = -INF
+    live = [0, 1, 3, 4, 5, 6, 7]
+    g = torch.randn((9, k), generator=torch.Generator().manual_seed(1)).cuda()
+    leaf = x.clone().requires_grad_()
+    idx, w = pkg.route_experts(leaf, k, score=score, renormalize=renormalize, scale=1.5)
+    (w * g).sum().backward()
+    assert (idx[[2, 8]] == -1).all() and (w.detach()[[2, 8]] == 0).all()
+    assert (leaf.grad[[2, 8]] == 0).all()
+    alone = pkg.route_experts_backward(g[live], x[live], idx[live], score=score, renormalize=renormalize, scale=1.5)
+    assert torch.equal(leaf.grad[live], alone) and torch.isfinite(alone.float()).all()
+    # a row whose places are all -1 is a constant whatever its logits are
+    none = torch.full_like(idx, -1)
+    assert (pkg.route_experts_backward(g, x, none, score=score, renormalize=renormalize) == 0).all()
+    ref = X.route_grad(g.cpu().numpy(), x.double().cpu().numpy(), idx.cpu().numpy(), score, renormalize, 1.5)
+    assert (ref[[2, 8]] == 0).all()
+
+
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_gradient_shows_a_nan_logit(pkg, renormalize):
+    """A NaN among excluded experts is picked, so its row's gradient is NaN; other rows do not see it."""
+    x = torch.full((3, 64), -INF, device="cuda")
+    x[0, :8] = x[2, :8] = torch.arange(8.0, device="cuda")
+    x[1, 5] = float("nan")
+    leaf = x.requires_grad_()
+    idx, w = pkg.route_experts(leaf, 4, renormalize=renormalize)
+    assert idx[1].tolist() == [5, -1, -1, -1]
+    w.sum().backward()
+    assert torch.isnan(leaf.grad[1]).any() and torch.isfinite(leaf.grad[[0, 2]]).all()
