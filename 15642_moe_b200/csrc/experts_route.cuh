@@ -9,8 +9,9 @@
  *   idx    = the top_k best picks, descending, ties to the lower expert; -1 where no expert is left
  *   w      = scale * s[idx], divided by (sum of the row's picked s + 1e-20) if renormalised; 0 for idx -1
  *
- * Without a bias the scores keep the logits' order, so the logits themselves are compared: experts whose
- * scores round to the same 32-bit value are still told apart, and no exponential is spent on the choice.
+ * Without a bias the scores keep the logits' order, so experts are compared by their logits: those whose
+ * scores round to the same 32-bit value are still told apart. Only sums of two scores (group_top2) need
+ * exponentials for the choice then; groups whose sums round together go by their order.
  *
  * One warp per token, VPT = ceil(E / 32) neighbouring experts per lane in registers. The choice:
  *   1. each lane's best key; k rounds of (warp maximum, lanes holding it drop out) give a key that at
@@ -237,6 +238,12 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
       for (int i = 0; i < VPT; ++i)
         if (first + i < p.E && ((dropped >> ((first + i) / per)) & 1u)) key[i] = RX_NONE;
     }
+  }
+
+  // Without a bias the kept groups' experts are compared by their logits; the scores were for the groups' sums alone.
+  if (p.bias == nullptr && !by_logit) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) key[i] = key[i] == RX_NONE ? RX_NONE : pick_key(x[i]);
   }
 
   // 1. A key that at least k experts reach (or all that are left).

@@ -46,3 +46,27 @@ def test_gradient_shows_a_nan_logit(pkg, renormalize):
     assert idx[1].tolist() == [5, -1, -1, -1]
     w.sum().backward()
     assert torch.isnan(leaf.grad[1]).any() and torch.isfinite(leaf.grad[[0, 2]]).all()
+
+
+def _same_order(pkg, x, k, bias=None, **rule):
+    idx, _ = pkg.route_experts(x, k, bias=bias, **rule)
+    score = rule.pop("score")
+    ref, _ = X.route(x.double().cpu().numpy(), k, score, None if bias is None else bias.double().cpu().numpy(), **rule)
+    np.testing.assert_array_equal(idx.cpu().numpy(), ref)
+
+
+@pytest.mark.parametrize("E", [64, 48])
+def test_scores_that_round_together_without_a_bias(pkg, E):
+    """Without a bias the kept groups' experts are ordered by their logits, also where 32-bit scores are equal: sigmoids of
+    18 and more are 1, exponentials 110 below the maximum are 0. The groups themselves are far apart."""
+    rng, per = np.random.default_rng(E), E // 8
+    x = np.full((20, 8, per), -5.0, np.float32) - np.arange(8, dtype=np.float32)[:, None]
+    for t in range(20):
+        x[t, :4] = rng.permutation(np.linspace(18.0, 30.0, 4 * per)).reshape(4, per)
+    group = dict(n_group=8, topk_group=4, group_score="top2")
+    _same_order(pkg, torch.from_numpy(x.reshape(20, E)).cuda(), 12, score="sigmoid", **group)
+    for t in range(20):
+        x[t, :4] = -rng.permutation(np.linspace(110.0, 130.0, 4 * per)).reshape(4, per)
+        x[t, 4:] = -200.0
+        x[t, :4, 0] = [0.0, -0.5, -1.0, -1.5]
+    _same_order(pkg, torch.from_numpy(x.reshape(20, E)).cuda(), 12, score="softmax", **group)
