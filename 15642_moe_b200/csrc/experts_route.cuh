@@ -103,16 +103,12 @@ __device__ __forceinline__ void load_row(const T* row, int first, int E, bool ve
   }
 }
 
-// Scores for the choice: the hardware's 2^x and 1/x (relative errors below 2^-21 for logits of any size that matter). The
-// weights use expf.
-__device__ __forceinline__ float exp_fast(float x) {
+// Sigmoid of the choice, in 32 bits: expf (2 units of 2^-23 of its value at most), a sum and the hardware's 1/x (one
+// unit); below 2^-126 it is 0. ex2.approx of x log2(e) in its place loses |x| / 8 units by rounding the product: at |x| = 12
+// neighbouring float32 logits got one score.
+__device__ __forceinline__ float sigmoid_choice(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
-  return y;
-}
-__device__ __forceinline__ float sigmoid_fast(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + exp_fast(-x)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + expf(-x)));
   return y;
 }
 
@@ -151,7 +147,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     mx = warp_max(mx);
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) sum += exp_fast(x[i] - mx);
+    for (int i = 0; i < VPT; ++i) sum += expf(x[i] - mx);
     inv = 1.0f / warp_sum(sum);
   }
   const bool grouped = p.n_group > 1;
@@ -171,7 +167,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const float v = __fadd_rn(p.softmax ? exp_fast(x[i] - mx) * inv : sigmoid_fast(x[i]), b[i]);
+      const float v = __fadd_rn(p.softmax ? expf(x[i] - mx) * inv : sigmoid_choice(x[i]), b[i]);
       key[i] = x[i] == -INFINITY ? RX_NONE : pick_key(v);
     }
   }
@@ -324,9 +320,9 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_kernel(const __gr
   }
 
   float s = 0.0f;
-  if (my_idx >= 0) s = p.softmax ? expf(my_x - mx) * inv : __fdividef(1.0f, 1.0f + expf(-my_x));
+  if (my_idx >= 0) s = p.softmax ? expf(my_x - mx) * inv : 1.0f / (1.0f + expf(-my_x));
   if (p.renormalize) {
-    s = __fdividef(s, warp_sum(s) + 1e-20f);
+    s = s / (warp_sum(s) + 1e-20f);
   }
   if (place < p.k) {
     p.idx[t * p.k + place] = my_idx;
@@ -391,7 +387,7 @@ __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_backward_kernel(c
     }
     inv = 1.0f / warp_sum(sum);
   }
-  const float ex = expf(-fabsf(l)), r1 = __fdividef(1.0f, 1.0f + ex);
+  const float ex = expf(-fabsf(l)), r1 = 1.0f / (1.0f + ex);
   const float s = e < 0 ? 0.0f : p.softmax ? expf(l - mx) * inv : (l >= 0.0f ? r1 : ex * r1);
   const float gs = warp_sum(g * s);
   float d = g, dot = gs;

@@ -70,3 +70,30 @@ def test_scores_that_round_together_without_a_bias(pkg, E):
         x[t, 4:] = -200.0
         x[t, :4, 0] = [0.0, -0.5, -1.0, -1.5]
     _same_order(pkg, torch.from_numpy(x.reshape(20, E)).cuda(), 12, score="softmax", **group)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("base", [-9.0, -13.0, -15.5, -20.0, -29.0, -50.0])
+def test_choice_by_scores_of_32_bits(pkg, base, grouped, score):
+    """Neighbouring float32 logits around `base`, in any order, under a bias of zero, so that the scores are compared. They
+    are 2^-20 (8 to 16), 2^-19 or 2^-18 (32 to 64) apart, which is as much between their scores: 8 units of 2^-23 at least.
+    An exponential of 2 units, a sum of half a unit and a reciprocal or product of one are 7 for the two of them."""
+    rng, E = np.random.default_rng(0), 64
+    step = np.spacing(np.float32(abs(base)))
+    x = np.stack([base - 40 * step * t + step * rng.permutation(E) for t in range(30)]).astype(np.float32)
+    assert (np.diff(np.sort(x, 1), axis=1) == step).all()
+    group = dict(n_group=8, topk_group=8, group_score="top2") if grouped else {}
+    if score == "softmax":
+        x[:, 7] = 0.0
+    _same_order(pkg, torch.from_numpy(x).cuda(), 16, torch.zeros(E, device="cuda"), score=score, **group)
+
+
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_weights_of_32_bits(pkg, renormalize):
+    """Sigmoid weights. Units of 2^-24: exponential 4, sum 1, quotient 1, so 6 of a score. Without renormalisation 1 more for
+    the scale. With it the row's sum has the scores' 6 and 5 additions, then a quotient and the scale: 19."""
+    x = (3 * torch.randn((4096, 64), generator=torch.Generator().manual_seed(0))).cuda()
+    idx, w = pkg.route_experts(x, 6, score="sigmoid", renormalize=renormalize, scale=2.5)
+    ref = X.weights(X.scores(x.double().cpu().numpy(), "sigmoid"), idx.cpu().numpy(), renormalize, 2.5)
+    assert (np.abs(w.double().cpu().numpy() / ref - 1) <= (19 if renormalize else 7) * 2.0 ** -24).all()
