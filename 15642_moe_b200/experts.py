@@ -172,6 +172,26 @@ class _RouteExperts(torch.autograd.Function):
 
 
 # ----------------------------------------------------------------------------- 4-bit products
+class _NoGradient(torch.autograd.Function):
+    """A product whose backward pass fails, as for torch's own operators without a derivative: a result without a graph
+    would cut the gradient in silence."""
+
+    @staticmethod
+    def forward(ctx, name, product, *inputs):
+        ctx.name = name
+        return product()
+
+    @staticmethod
+    def backward(ctx, *_):
+        _fail(f"{ctx.name} has no gradient: give it detached tensors, or call it under torch.no_grad()")
+
+
+def _without_gradient(name, out, product, *inputs):
+    if out is not None:
+        _fail(f"{name} has no gradient: out= takes no inputs that require one")
+    return _NoGradient.apply(name, product, *inputs)
+
+
 def _w4(codes, scale, zero, group, shape, K, dtype, index, name) -> None:
     """Checks one 4-bit matrix (or a stack of them): `shape` without the columns, K columns."""
     if not (codes.dtype == torch.uint8 and codes.shape == (*shape, (K + 1) // 2) and codes.is_contiguous()):
@@ -209,7 +229,10 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: t
     """x [M, K] (bfloat16 or float16, rows any distance apart) times the 4-bit W [N, K]: [M, N] in x's type.
 
     ``codes``, ``scale``, ``zero`` as in this module's description, ``group`` 32, 64 or 128. M up to 65535, any N and
-    K from 1 on. ``out`` may not overlap an input. Sums are held in 32 bits and rounded once."""
+    K from 1 on. ``out`` may not overlap an input. Sums are held in 32 bits and rounded once. There is no gradient: where
+    ``x`` or ``scale`` requires one, the call works and a backward pass through its result raises ``RuntimeError``."""
+    if (x.requires_grad or scale.requires_grad) and torch.is_grad_enabled():
+        return _without_gradient("linear_w4", out, lambda: linear_w4(x, codes, scale, zero, group=group), x, scale)
     _check_x(x, group, "[M, K]")
     if codes.dim() != 2:
         _fail("codes must be [N, ceil(K / 2)]")
@@ -253,7 +276,12 @@ def experts_w4(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w13: t
     ``x`` [T, H] bfloat16 or float16, rows any distance apart; ``idx`` int32 and ``weights`` fp32 [T, top_k], as
     route_experts returns them; ``w13`` codes uint8 [E, 2 I, ceil(H / 2)], ``w2`` codes uint8 [E, H, ceil(I / 2)]
     (16-byte aligned), scales and zero points as in this module's description. T up to 65535. ``out`` may not overlap an
-    input. Sums are held in 32 bits and rounded once."""
+    input. Sums are held in 32 bits and rounded once. There is no gradient: where ``x``, ``weights`` or a scale requires
+    one, the call works and a backward pass through its result raises ``RuntimeError``."""
+    if (x.requires_grad or weights.requires_grad or w13_scale.requires_grad or w2_scale.requires_grad) and torch.is_grad_enabled():
+        return _without_gradient("experts_w4", out, lambda: experts_w4(
+            x, idx, weights, w13, w13_scale, w2, w2_scale, w13_zero=w13_zero, w2_zero=w2_zero, group=group,
+            local_offset=local_offset, workspace=workspace), x, weights, w13_scale, w2_scale)
     _check_x(x, group, "[T, H]")
     if not (w13.dim() == 3 and w13.shape[1] % 2 == 0):
         _fail("w13 must be [E, 2 I, ceil(H / 2)]")
