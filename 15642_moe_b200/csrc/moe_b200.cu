@@ -702,6 +702,9 @@ bool w4_rows_aligned(const void* codes, int K) { return w4_bytes(K) % 16 == 0 &&
 int wm_tile(long long rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 constexpr int WM_MAX_ROWS = 65535;   // rows of x: a grid dimension of the kernels around the products
+// Rows and columns of a matrix: rounded up to whole steps and tiles they stay inside 32 bits. The experts' combine walks 4096
+// columns at a time.
+constexpr int W4_MAX_DIM = 0x7FFFFFFF - 255, W4_MAX_WIDTH = 1 << 30;
 constexpr int WM_SMS = 148;   // the split rule's SM count: results and workspace sizes do not depend on the device
 
 // linear_w4: parts of the columns, so that few row tiles still fill the SMs; two steps each at least.
@@ -995,7 +998,7 @@ int moe_route_experts_backward(const moe_route_experts_backward_args* args) {
 }
 
 size_t moe_linear_w4_workspace_bytes(int M, int N, int K) {
-  if (M <= WS_TOK || N < 1 || K < 1) return 0;
+  if (M <= WS_TOK || M > WM_MAX_ROWS || N < 1 || N > W4_MAX_DIM || K < 1 || K > W4_MAX_DIM) return 0;
   return make_linear_w4_ws(M, N, K).total;
 }
 
@@ -1004,6 +1007,7 @@ int moe_linear_w4(const moe_linear_w4_args* args) {
   const auto [x, codes, scale, zero, out, workspace, stream, x_stride, workspace_bytes, dtype, group, M, N, K] = *args;
   if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be bf16 or f16");
   if (M < 0 || N < 1 || K < 1) return fail(MOE_ERR_INVALID, "moe_linear_w4: x must be [M, K] and W [N, K]");
+  if (N > W4_MAX_DIM || K > W4_MAX_DIM) return fail(MOE_ERR_INVALID, "moe_linear_w4: N and K must be at most 2^31 - 256");
   if (M > WM_MAX_ROWS || static_cast<long long>(M) * round_up(K, 64) > 0x7FFFFFFFll)
     return fail(MOE_ERR_INVALID, "moe_linear_w4: M must be at most 65535, and x have less than 2^31 elements");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_linear_w4: group must be 32, 64 or 128");
@@ -1029,7 +1033,9 @@ int moe_linear_w4(const moe_linear_w4_args* args) {
 }
 
 size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I) {
-  if (T < 0 || T > WM_MAX_ROWS || top_k < 1 || top_k > RX_MAX_K || E < 1 || E > RX_MAX_E || H < 1 || I < 1) return 0;
+  if (T < 0 || T > WM_MAX_ROWS || top_k < 1 || top_k > RX_MAX_K || E < 1 || E > RX_MAX_E || H < 1 || I < 1 || H > W4_MAX_WIDTH ||
+      I > W4_MAX_WIDTH)
+    return 0;
   return make_experts_w4_ws(T, top_k, E, H, I).total;
 }
 
@@ -1041,7 +1047,8 @@ int moe_experts_w4(const moe_experts_w4_args* args) {
   if (T < 0 || T > WM_MAX_ROWS) return fail(MOE_ERR_INVALID, "moe_experts_w4: T must be 0 to 65535");
   if (top_k < 1 || top_k > RX_MAX_K) return fail(MOE_ERR_INVALID, "moe_experts_w4: top_k must be 1 to 32");
   if (E < 1 || E > RX_MAX_E) return fail(MOE_ERR_INVALID, "moe_experts_w4: E must be 1 to 1024");
-  if (H < 1 || I < 1) return fail(MOE_ERR_INVALID, "moe_experts_w4: H and I must be at least 1");
+  if (H < 1 || I < 1 || H > W4_MAX_WIDTH || I > W4_MAX_WIDTH)
+    return fail(MOE_ERR_INVALID, "moe_experts_w4: H and I must be 1 to 2^30");
   if (static_cast<long long>(E) * (2ll * I > H ? 2ll * I : H) > 0x7FFFFFFFll)
     return fail(MOE_ERR_INVALID, "moe_experts_w4: the experts' matrices have more than 2^31 rows");
   if (group != 32 && group != 64 && group != 128) return fail(MOE_ERR_INVALID, "moe_experts_w4: group must be 32, 64 or 128");

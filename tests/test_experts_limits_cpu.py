@@ -1,0 +1,50 @@
+"""Host side of the expert operators at the edges of what their integers hold. Nothing here launches a kernel."""
+import ctypes
+import importlib
+
+import pytest
+
+INT_MAX = 2 ** 31 - 1
+
+
+@pytest.fixture(scope="module")
+def lib(pkg):
+    return importlib.import_module("15642_moe_b200._native").cuda_lib()
+
+
+@pytest.fixture(scope="module")
+def ex(pkg):
+    return importlib.import_module("15642_moe_b200.experts")
+
+
+@pytest.fixture(scope="module")
+def p():
+    buf = (ctypes.c_uint8 * 4096)()
+    yield (ctypes.addressof(buf) + 255) & ~255
+
+
+def test_columns_beyond_the_limit_are_refused(lib, ex, p):
+    """Rounding a column count up to whole steps must stay inside 32 bits."""
+    far = 1 << 50                                                      # an output that overlaps nothing
+    linear = lambda M=2, N=8, K=64: lib.moe_linear_w4(  # noqa: E731
+        ex._LINEAR(p, p, p, 0, far, far // 2, 0, K, 1 << 62, 1, 128, M, N, K))
+    for M in (1, 8, 9, 65535):
+        for K in (INT_MAX, INT_MAX - 1, INT_MAX - 62, INT_MAX - 254):
+            assert linear(M=M, K=K) == 1 and b"moe_linear_w4" in lib.moe_last_error(), (M, K)
+            assert lib.moe_linear_w4_workspace_bytes(M, 8, K) == 0
+        assert linear(M=M, N=INT_MAX, K=2) == 1 and b"moe_linear_w4" in lib.moe_last_error()
+    experts = lambda E=1, H=64, I=64: lib.moe_experts_w4(  # noqa: E731
+        ex._EXPERTS(p, p, p, p, p, 0, p, p, 0, far, far // 2, 0, H, 1 << 62, 1, 128, 2, 2, E, 0, H, I))
+    for big in (INT_MAX, INT_MAX - 62, INT_MAX - 254, 2 ** 30 + 1):
+        for kw in (dict(H=big), dict(I=big)):
+            assert experts(**kw) == 1 and b"moe_experts_w4" in lib.moe_last_error(), kw
+        assert lib.moe_experts_w4_workspace_bytes(2, 2, 1, big, 64) == 0
+        assert lib.moe_experts_w4_workspace_bytes(2, 2, 1, 64, big) == 0
+
+
+def test_workspace_sizes_up_to_the_limit(lib):
+    """Sizes of widths that need no copy of the codes grow up to the largest that is taken."""
+    sizes = [lib.moe_linear_w4_workspace_bytes(9, 8, K) for K in (64, 4096, 2 ** 20, 2 ** 27)]
+    assert sizes == sorted(sizes) and sizes[0] > 0 and sizes[-1] >= 9 * 2 ** 27 * 2
+    sizes = [lib.moe_experts_w4_workspace_bytes(2, 2, 1, H, 64) for H in (64, 4096, 2 ** 20, 2 ** 30)]
+    assert sizes == sorted(sizes) and sizes[0] > 0 and sizes[-1] >= 4 * 2 ** 30 * (2 + 4)
