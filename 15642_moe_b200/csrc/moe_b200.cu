@@ -686,7 +686,7 @@ struct Span {
   const void* p;
   size_t n;
 };
-// Blocks write output rows while others still read inputs, so the output may overlap none of them.
+// Blocks write the output and the workspace while others still read inputs, so they may overlap none of them.
 bool overlaps(const void* out, size_t n, std::initializer_list<Span> in) {
   const uintptr_t o0 = reinterpret_cast<uintptr_t>(out), o1 = o0 + n;
   for (const Span& s : in) {
@@ -1023,9 +1023,11 @@ int moe_linear_w4(const moe_linear_w4_args* args) {
       return fail(MOE_ERR_INVALID, "moe_linear_w4: workspace must be 256-byte aligned");
   }
   const size_t m = static_cast<size_t>(M), groups = (static_cast<size_t>(K) + group - 1) / group, n = static_cast<size_t>(N);
-  if (overlaps(out, m * n * 2, {{x, row_bytes(M, x_stride, K)}, {codes, n * w4_bytes(K)}, {scale, n * groups * 2}, {zero, zero ? n * groups : 0},
-                                {workspace, moe_linear_w4_workspace_bytes(M, N, K)}}))
+  const size_t scratch = moe_linear_w4_workspace_bytes(M, N, K);
+  const auto in = {Span{x, row_bytes(M, x_stride, K)}, Span{codes, n * w4_bytes(K)}, Span{scale, n * groups * 2}, Span{zero, zero ? n * groups : 0}};
+  if (overlaps(out, m * n * 2, in) || overlaps(out, m * n * 2, {Span{workspace, scratch}}))
     return fail(MOE_ERR_INVALID, "moe_linear_w4: the output overlaps an input or the workspace");
+  if (scratch != 0 && overlaps(workspace, scratch, in)) return fail(MOE_ERR_INVALID, "moe_linear_w4: the workspace overlaps an input");
   DeviceInfo* d = nullptr;
   if (int rc = device_info(&d)) return rc;
   return dtype == MOE_BF16 ? linear_w4_impl<__nv_bfloat16>(d, x, x_stride, w, M, N, K, out, workspace, st)
@@ -1065,11 +1067,13 @@ int moe_experts_w4(const moe_experts_w4_args* args) {
   {
     const size_t e = static_cast<size_t>(E), picks = static_cast<size_t>(T) * top_k, h = static_cast<size_t>(H), i = static_cast<size_t>(I);
     const size_t g13 = (h + group - 1) / group, g2 = (i + group - 1) / group;
-    if (overlaps(out, static_cast<size_t>(T) * h * 2,
-                 {{x, row_bytes(T, x_stride, H)}, {idx, picks * 4}, {w, picks * 4}, {w13, e * 2 * i * w4_bytes(H)}, {w13_scale, e * 2 * i * g13 * 2},
-                  {w13_zero, w13_zero ? e * 2 * i * g13 : 0}, {w2, e * h * w4_bytes(I)}, {w2_scale, e * h * g2 * 2},
-                  {w2_zero, w2_zero ? e * h * g2 : 0}, {workspace, need}}))
+    const auto in = {Span{x, row_bytes(T, x_stride, H)}, Span{idx, picks * 4}, Span{w, picks * 4}, Span{w13, e * 2 * i * w4_bytes(H)},
+                     Span{w13_scale, e * 2 * i * g13 * 2}, Span{w13_zero, w13_zero ? e * 2 * i * g13 : 0}, Span{w2, e * h * w4_bytes(I)},
+                     Span{w2_scale, e * h * g2 * 2}, Span{w2_zero, w2_zero ? e * h * g2 : 0}};
+    if (overlaps(out, static_cast<size_t>(T) * h * 2, in) || overlaps(out, static_cast<size_t>(T) * h * 2, {Span{workspace, need}}))
       return fail(MOE_ERR_INVALID, "moe_experts_w4: the output overlaps an input or the workspace");
+    // The plan writes the workspace while idx is still read: picks that change in between would index past its tables.
+    if (overlaps(workspace, need, in)) return fail(MOE_ERR_INVALID, "moe_experts_w4: the workspace overlaps an input");
   }
   const ExpertsW4Args a{x, x_stride, idx, w,
                         {static_cast<const uint8_t*>(w13), w13_scale, static_cast<const uint8_t*>(w13_zero), group},

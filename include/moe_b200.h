@@ -246,7 +246,8 @@ int moe_route_experts_backward(const moe_route_experts_backward_args* args);
  * bits), or NULL for 8; group 32, 64 or 128. Weight = scale * (code - zero). Stacked matrices follow one another.
  *
  * moe_linear_w4: out [M, N] = x . W^T, x [M, K] with rows x_stride elements apart, out contiguous, M up to 65535, N and K up to 2^31 - 256
- * and x below 2^31 elements; both of type `dtype`; out may not overlap an input or the workspace. Sums in fp32, rounded once. The workspace (256-byte aligned) is needed above 8 tokens; below, its size is 0
+ * and x below 2^31 elements; both of type `dtype`; neither out nor the workspace may overlap an input,
+ * nor each other. Sums in fp32, rounded once. The workspace (256-byte aligned) is needed above 8 tokens; below, its size is 0
  * and it may be NULL. */
 size_t moe_linear_w4_workspace_bytes(int M, int N, int K);
 typedef struct {
@@ -260,8 +261,8 @@ int moe_linear_w4(const moe_linear_w4_args* args);
 /* Routed experts with 4-bit weights: for every token t and pick j whose expert e = idx[t, j] - local_offset is in
  * [0, E): out[t] += w[t, j] * W2[e] (X1 * silu(X2)), [X1 | X2] = W13[e] x[t]. x [T, H] with rows x_stride
  * elements apart; idx int32 and w fp32 [T, top_k]; w13 stacked [E, 2 I, H], w2 stacked [E, H, I]; out [T, H]
- * contiguous, of x's type (zeros for a token without a pick here). w13 and w2 16-byte, the workspace 256-byte aligned; out may
- * not overlap an input or the workspace; local_offset >= 0. 0 <= T <= 65535, top_k <= 32, E <= 1024, H and I up
+ * contiguous, of x's type (zeros for a token without a pick here). w13 and w2 16-byte, the workspace 256-byte aligned; neither
+ * out nor the workspace may overlap an input, nor each other; local_offset >= 0. 0 <= T <= 65535, top_k <= 32, E <= 1024, H and I up
  * to 2^30, E * H and E * 2 I below 2^31. */
 size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I);
 typedef struct {

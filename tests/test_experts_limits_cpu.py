@@ -48,3 +48,25 @@ def test_workspace_sizes_up_to_the_limit(lib):
     assert sizes == sorted(sizes) and sizes[0] > 0 and sizes[-1] >= 9 * 2 ** 27 * 2
     sizes = [lib.moe_experts_w4_workspace_bytes(2, 2, 1, H, 64) for H in (64, 4096, 2 ** 20, 2 ** 30)]
     assert sizes == sorted(sizes) and sizes[0] > 0 and sizes[-1] >= 4 * 2 ** 30 * (2 + 4)
+
+
+def test_a_workspace_over_an_input_is_refused(lib, ex, p):
+    """Every input in turn lies in the workspace's first or last bytes."""
+    far = lambda i: (1 << 50) + (i << 24)  # noqa: E731
+    M, N, K = 9, 8, 64
+    need = lib.moe_linear_w4_workspace_bytes(M, N, K)
+    ws = far(20)
+    for at in range(4):                                                # x, codes, scale, zero
+        for place in (ws, ws + need - 1):
+            a = [far(i) for i in range(4)]
+            a[at] = place
+            rc = lib.moe_linear_w4(ex._LINEAR(*a, far(10), ws, 0, K, need, 1, 32, M, N, K))
+            assert rc == 1 and b"workspace overlaps an input" in lib.moe_last_error(), at
+    T, k, E, H, I = 2, 2, 4, 64, 32
+    need = lib.moe_experts_w4_workspace_bytes(T, k, E, H, I)
+    for at in range(9):                                                # x, idx, weights, w13, scale, zero, w2, scale, zero
+        for place in (ws, ws + need // 256 * 256 - 256):
+            a = [far(i) for i in range(9)]
+            a[at] = place
+            rc = lib.moe_experts_w4(ex._EXPERTS(*a, far(10), ws, 0, H, need, 1, 32, T, k, E, 0, H, I))
+            assert rc == 1 and b"workspace overlaps an input" in lib.moe_last_error(), at
