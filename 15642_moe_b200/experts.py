@@ -39,7 +39,8 @@ def _native_lib():
     return _lib
 
 
-# The argument structs of include/moe_b200.h.
+# The argument structs of include/moe_b200.h, up to their last member, and the padding that may follow it.
+_TAIL = bytes(4)
 _ROUTE = struct.Struct("@5Pq9if").pack
 _ROUTE_BACKWARD = struct.Struct("@5Pq6if").pack
 _LINEAR = struct.Struct("@7P2q5i").pack
@@ -48,6 +49,7 @@ _EXPERTS = struct.Struct("@12P2q8i").pack
 
 def _call(fn, index: int, args: bytes) -> None:
     """One C call with device `index` current."""
+    args += _TAIL
     if index == torch.cuda.current_device():
         rc = fn(args)
     else:

@@ -70,3 +70,15 @@ def test_a_workspace_over_an_input_is_refused(lib, ex, p):
             a[at] = place
             rc = lib.moe_experts_w4(ex._EXPERTS(*a, far(10), ws, 0, H, need, 1, 32, T, k, E, 0, H, I))
             assert rc == 1 and b"workspace overlaps an input" in lib.moe_last_error(), at
+
+
+def test_calls_hand_over_whole_structs(ex, monkeypatch):
+    """The C side copies its struct, padding at the end included: the bytes handed over must be as many."""
+    P, L, I, F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
+    monkeypatch.setattr(ex.torch.cuda, "current_device", lambda: 0)
+    for pack, members in ((ex._ROUTE, [P] * 5 + [L] + [I] * 9 + [F]), (ex._ROUTE_BACKWARD, [P] * 5 + [L] + [I] * 6 + [F]),
+                          (ex._LINEAR, [P] * 7 + [L] * 2 + [I] * 5), (ex._EXPERTS, [P] * 12 + [L] * 2 + [I] * 8)):
+        layout = type("Args", (ctypes.Structure,), {"_fields_": [("m%d" % i, t) for i, t in enumerate(members)]})
+        args, seen = pack(*(1.5 if t is F else i for i, t in enumerate(members))), []
+        ex._call(lambda a: seen.append(a) or 0, 0, args)
+        assert len(seen[0]) >= ctypes.sizeof(layout) and seen[0].startswith(args)
