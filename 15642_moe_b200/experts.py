@@ -13,6 +13,7 @@ several experts are stacked in a leading dimension.
 from __future__ import annotations
 
 import functools
+import operator
 import struct
 
 import torch
@@ -22,6 +23,7 @@ from . import _native
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SCORE = {"sigmoid": 0, "softmax": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
+_SCORES, _GROUP_SCORES = tuple(_SCORE), tuple(_GROUP_SCORE)
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS, MAX_ROWS = 1024, 32, 32, 65535
 W4_GROUPS = (32, 64, 128)
 
@@ -63,6 +65,19 @@ def _fail(message: str) -> None:
     raise RuntimeError(message)
 
 
+def _whole(name: str, value) -> int:
+    try:
+        return operator.index(value)
+    except TypeError:
+        _fail(f"{name} must be a whole number")
+
+
+def _scale(value) -> float:
+    if not hasattr(value, "__float__"):
+        _fail("scale must be a number")
+    return float(value)
+
+
 # ------------------------------------------------------------------------------------ router
 # The messages are built only where a check fails: a call is a few microseconds in all.
 def _check_logits(logits) -> None:
@@ -100,10 +115,12 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         return _RouteExperts.apply(logits, top_k, score, bias, n_group, topk_group, group_score, renormalize, scale)
     _check_logits(logits)
     T, E = logits.shape
-    if score not in _SCORE:
+    if score not in _SCORES:
         _fail("score must be 'softmax' or 'sigmoid'")
-    if group_score not in _GROUP_SCORE:
+    if group_score not in _GROUP_SCORES:
         _fail("group_score must be 'max' or 'top2'")
+    if not type(top_k) is type(n_group) is type(topk_group) is int:
+        top_k, n_group, topk_group = _whole("top_k", top_k), _whole("n_group", n_group), _whole("topk_group", topk_group)
     if not (1 <= n_group <= MAX_GROUPS and E % n_group == 0):
         _fail(f"n_group must divide the experts and be 1 to {MAX_GROUPS}")
     if not 1 <= topk_group <= n_group:
@@ -124,7 +141,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         _call(_native_lib().moe_route_experts, index,
               _ROUTE(logits.data_ptr(), bias_ptr, idx.data_ptr(), w.data_ptr(), _current_stream(index), logits.stride(0),
                      _DTYPE[logits.dtype], T, E, top_k, _SCORE[score], n_group, topk_group, _GROUP_SCORE[group_score],
-                     bool(renormalize), scale))
+                     bool(renormalize), scale if type(scale) is float else _scale(scale)))
     return idx, w
 
 
@@ -137,7 +154,7 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, idx
     experts has no gradient."""
     _check_logits(logits)
     T, E = logits.shape
-    if score not in _SCORE:
+    if score not in _SCORES:
         _fail("score must be 'softmax' or 'sigmoid'")
     index = logits.get_device()
     if not (idx.dim() == 2 and idx.shape[0] == T and 1 <= idx.shape[1] <= MAX_TOP_K and idx.dtype == torch.int32
@@ -151,7 +168,7 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, idx
         _call(_native_lib().moe_route_experts_backward, index,
               _ROUTE_BACKWARD(grad_weights.data_ptr(), logits.data_ptr(), idx.data_ptr(), grad.data_ptr(),
                               _current_stream(index), logits.stride(0), _DTYPE[logits.dtype], T, E, idx.shape[1],
-                              _SCORE[score], bool(renormalize), scale))
+                              _SCORE[score], bool(renormalize), scale if type(scale) is float else _scale(scale)))
     return grad
 
 
@@ -215,7 +232,7 @@ def _check_x(x, group, what) -> None:
         _fail("x must be bfloat16 or float16")
     if not x.is_cuda:
         _fail("x must be a CUDA tensor")
-    if group not in W4_GROUPS:
+    if group not in W4_GROUPS or type(group) is float:
         _fail("group must be 32, 64 or 128")
     if x.shape[0] > 0 and x.shape[1] > 1 and x.stride(1) != 1:
         _fail("x must have neighbouring columns in memory (stride 1)")
@@ -261,7 +278,9 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: t
 
 @functools.lru_cache(maxsize=4096)
 def experts_w4_workspace_bytes(T: int, top_k: int, E: int, H: int, I: int) -> int:
-    """Bytes of experts_w4's workspace."""
+    """Bytes of experts_w4's workspace; 0 for sizes that it refuses."""
+    if max(T, top_k, E, H, I) >= 2 ** 31 or min(T, top_k, E, H, I) < 0:
+        return 0
     return int(_native_lib().moe_experts_w4_workspace_bytes(T, top_k, E, H, I))
 
 
@@ -293,6 +312,8 @@ def experts_w4(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w13: t
         _fail(f"w13 must hold 1 to {MAX_EXPERTS} experts")
     if T > MAX_ROWS:
         _fail(f"x must have at most {MAX_ROWS} tokens")
+    if not 0 <= _whole("local_offset", local_offset) < 2 ** 31:
+        _fail("local_offset must be 0 to 2^31 - 1")
     if not (idx.dim() == 2 and idx.shape[0] == T and 1 <= idx.shape[1] <= MAX_TOP_K and idx.dtype == torch.int32
             and idx.is_contiguous() and idx.is_cuda and idx.get_device() == index):
         _fail(f"idx must be a contiguous int32 [T, top_k] tensor on x's device, top_k 1 to {MAX_TOP_K}")
