@@ -21,10 +21,10 @@
  * More than 32 candidates (many equal scores, or the best ones side by side in a few lanes): k rounds of
  * arg-max over the warp instead, with the same result.
  *
- * Measured on a B200 (device time): 16384 tokens, 256 experts, sigmoid, bias, 8 groups, top 8: 13.2 us, 1.3 TB/s of
- * logits; 3.8 us for 4096 tokens without groups and bias; one token 2.7 us. Bound by instructions (three
- * quarters of the issue slots at 16384 tokens), not by memory: the floor there is 2.8 us. The first version,
- * with accurate exponentials for the choice and one lane per group, took 34 us.
+ * Measured on a B200 (device time): 16384 tokens, 256 experts, sigmoid, bias, 8 groups, top 8: 14.4 us, 1.2 TB/s of
+ * logits; 4.0 us for 4096 tokens without groups and bias; one token 3.1 us. Bound by instructions (771 per token and
+ * 76% of the issue slots at 16384 tokens: profiles/route_experts_t16384.md), not by memory: the floor there is
+ * 2.8 us. With ex2.approx for the choice it took 13.2 us, and neighbouring logits got one score.
  */
 #pragma once
 #include "moe_common.cuh"
@@ -351,7 +351,8 @@ struct RouteExpertsBwdArgs {
  * The choice itself (idx) has no gradient, nor has the bias.
  *
  * A row is written twice where it was picked: first every expert's value without a pick, then the picks over it. That
- * needs no shared memory (7.0 us either way at 16384 x 256, sigmoid; the floor is 2.8 us, most of it the dense output).
+ * needs no shared memory (which took as long). 6.8 us at 16384 x 256, sigmoid; the floor is 2.8 us, most of it the dense
+ * output. Half of a warp's time is waiting for loads (the picks, then their logits) before its first store.
  */
 template <typename T, int VPT>
 __global__ void __launch_bounds__(32 * RX_WARPS) route_experts_backward_kernel(const __grid_constant__ RouteExpertsBwdArgs p) {

@@ -698,7 +698,9 @@ bool overlaps(const void* out, size_t n, std::initializer_list<Span> in) {
 // TMA wants rows that start on 16-byte boundaries.
 bool w4_rows_aligned(const void* codes, int K) { return w4_bytes(K) % 16 == 0 && aligned16(codes); }
 
-// Tokens per tile: the accumulators are as small as the largest expected tile allows, so that more of them fit.
+// Tokens per tile: the accumulators are as small as the largest expected tile allows, so that more of them fit. For the experts
+// `rows` are the picks per expert of this GPU, those of other GPUs among them (their number is not known on the host): a
+// slice of a layer gets tiles that are too large, at 32 of 256 experts by up to eight times.
 int wm_tile(long long rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 constexpr int WM_MAX_ROWS = 65535;   // rows of x: a grid dimension of the kernels around the products

@@ -16,15 +16,12 @@
  * steps of 256 columns; one or two scale and store. Persistent: one block per SM walks
  * the units (token tile, 128 weight rows[, part of the columns]).
  *
- * Measured on a B200 (device time, 32 experts of 7168 x 2048, group 128): T = 64 of a 256-expert layer 188 us, 3.3 TB/s of
- * weights; T = 4096 742 to 745 us, 485 TFLOP/s; linear_w4 512 x 4096 x 7168 39 us, 770 TFLOP/s. What bounds it, by leaving parts
- * out: T = 64 took 182 us whole, 159 without the conversion, 168 without the mma, 170 without the scaling, 143 without
- * conversion and its stores, about what loading the weights and the waves of units take. Leaving out parts shifts the other
- * roles' waits too (199 us without the stores alone), so these bound the shares and do not add up. T = 4096 took 749 us whole,
- * 683 to 758 without one of the first three and 808 without the stores alone, so none of them alone is the limit. What is left
- * is the way into the SM: a step brings 16 KB of codes and up to 64 KB of token rows, which at 64 bytes a cycle (reckoned,
- * not measured by itself) is as long as its mma. Pairs of SMs that share the token rows
- * (cta_group::2) would halve that.
+ * Measured on a B200 (device time, 32 experts of 7168 x 2048, group 128): T = 64 of a 256-expert layer 187 us, 3.3 TB/s of
+ * weights; T = 4096 742 us, 485 TFLOP/s; linear_w4 512 x 4096 x 7168 39 us, 770 TFLOP/s. Counters (profiles/w4_mma.md): T = 64's
+ * first product keeps DRAM 42%, the issue slots 59% and the tensor pipe 10% busy, T = 4096's 22%, 55% and 34%: nothing is
+ * full, the roles wait for each other. At T = 4096 the likely reason is the way into the SM: a step brings 16 KB of codes
+ * and up to 64 KB of token rows, which at 64 bytes a cycle (reckoned, not measured by itself) is as long as its mma. Pairs
+ * of SMs that share the token rows (cta_group::2) would halve that.
  */
 #pragma once
 #include "gate.cuh"
@@ -600,7 +597,8 @@ __global__ void __launch_bounds__(WmShape<NT, MODE == WS_DOWN ? 2 : 1, G>::THREA
         }
       } else {
         // Lanes 0-15 hold X1, lanes 16-31 X2 of the same columns: even tokens end in the first, odd in the second.
-        // hi + lo bf16 carry 16 bits of h; the columns go in pair order, zeros up to the next 64.
+        // hi + lo bf16 carry 16 bits of h (off by 2^-17 at most; one term, off by 2^-8, would add as much as the output's own
+        // rounding, and f16 terms would overflow); the columns go in pair order, zeros up to the next 64.
         const int pos = pair_pos(col), mine = lane >> 4;
 #pragma unroll
         for (int i = 0; i < TOK; i += 2)

@@ -7,8 +7,8 @@
  * A thread holds, of rows g and g + 8 of a tile, the codes at a few places; which columns those are is free as long as A
  * and B agree. Thread t of a row's four takes group / 4 neighbouring columns of each group (one 16-, 8- or 4-byte load); a
  * 32-bit word of 8 codes makes the fragments of two mma. Codes become numbers by placing a nibble in the mantissa of 128
- * (bf16) or 1024 (f16) and subtracting 128 + zero or 1024 + zero: exact, as is every product. Each group's sum is scaled in
- * fp32: no weight is rounded.
+ * (bf16) or 1024 (f16) and subtracting 128 + zero or 1024 + zero: exact, as is every product (published for f16 by Kim et
+ * al., "Who Says Elephants Can't Run", 2022). Each group's sum is scaled in fp32: no weight is rounded.
  *
  * Split: a block has one tile of 16 rows, its 8 warps an eighth of the columns each; their sums meet in shared memory in
  * warp order, so results repeat bit for bit. Nothing is staged: a warp alone uses its columns of x. 1 to 4 steps of 128
@@ -16,10 +16,13 @@
  *
  * Measured on a B200 (device time, group 128): 4096 x 7168 for one token 8.5 to 9.6 us, from one B200 to another (1.5 to
  * 1.7 TB/s of codes; three copies of the weights in turn, which L2 holds), for 8 tokens 9.9 us; 7168 x 2048 6.2 us;
- * 28672 x 7168, which L2 does not hold so, 47.8 us (2.1 TB/s), for 8 tokens 55.7 us. Bound by instructions: about 19 per 256 weights, of which the
- * conversion has 11. An e4m3 mma would need no conversion (a code's byte is an e4m3 number), but mma.sync with it
- * took some 30 issue slots on sm_100a, more than the conversion. Staging activations and scales in
- * shared memory, with the columns split over a cluster, took 14 us for the first shape.
+ * 28672 x 7168, which L2 does not hold so, 47.6 us (2.2 TB/s), for 8 tokens 55.6 us. No single part is the limit there
+ * (profiles/w4_stream_m1.md): 36 instructions per 256 weights take 56% of the issue slots, DRAM is 25% busy, and with 4
+ * warps to a scheduler (128 registers) the slots left empty are waits for memory, for the instruction before and for the
+ * arithmetic pipes, in this order. A block's 7 steps per warp begin with an empty pipe each time. An e4m3 mma would need
+ * no conversion (a code's byte is an e4m3 number), but mma.sync with it took some 30 issue slots on sm_100a, more than the
+ * conversion. Staging activations and scales in shared memory, with the columns split over a cluster, took 14 us for the
+ * first shape.
  */
 #pragma once
 #include "gate.cuh"

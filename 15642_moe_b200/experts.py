@@ -106,7 +106,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     ``idx`` is in descending order of the choice, ties to the lower expert. Experts with a logit (or bias) of -inf
     are never chosen; where a row has fewer than top_k experts left, idx is -1 and the weight 0. The weights are
     divided by their sum (plus 1e-20) if ``renormalize``, then multiplied by ``scale``. A NaN logit comes out as
-    NaN weights. Differentiable in ``logits`` (route_experts_backward).
+    NaN weights. Scores, weights and their sums are in 32 bits; without a bias experts are compared by their logits, so those
+    whose scores round together keep their order. Differentiable in ``logits`` (route_experts_backward); the choice, and with
+    it the bias, has no gradient.
 
     The fixed router of moe_forward (reference/moe_ref.py:82-107) is score="sigmoid", n_group=8, topk_group=4,
     group_score="top2", top_k=8 over 256 experts.
@@ -150,8 +152,8 @@ def route_experts_backward(grad_weights: torch.Tensor, logits: torch.Tensor, idx
     """Gradient of route_experts' weights with respect to the logits: [T, E] in the logits' type.
 
     ``grad_weights`` fp32 [T, top_k], ``idx`` int32 [T, top_k] as route_experts returned it (distinct experts per
-    row; -1 takes no part), and the forward call's ``score``, ``renormalize`` and ``scale``. The choice of the
-    experts has no gradient."""
+    row; -1 takes no part, and a row of -1 alone has a zero gradient), and the forward call's ``score``, ``renormalize`` and
+    ``scale``. The choice of the experts has no gradient. The result itself is not differentiable."""
     _check_logits(logits)
     T, E = logits.shape
     if score not in _SCORES:
@@ -297,7 +299,9 @@ def experts_w4(x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, w13: t
     ``x`` [T, H] bfloat16 or float16, rows any distance apart; ``idx`` int32 and ``weights`` fp32 [T, top_k], as
     route_experts returns them; ``w13`` codes uint8 [E, 2 I, ceil(H / 2)], ``w2`` codes uint8 [E, H, ceil(I / 2)]
     (16-byte aligned), scales and zero points as in this module's description. T up to 65535. ``out`` may not overlap an
-    input. Sums are held in 32 bits and rounded once. There is no gradient: where ``x``, ``weights`` or a scale requires
+    input. Each product's sums and the weighted sum are held in 32 bits and the result is rounded once; between the products
+    the SwiGLU's result carries 16 bits (two bfloat16 terms: an error of at most 2^-17 of each value, where a bfloat16 output
+    is rounded by up to 2^-8). There is no gradient: where ``x``, ``weights`` or a scale requires
     one, the call works and a backward pass through its result raises ``RuntimeError``."""
     if (x.requires_grad or weights.requires_grad or w13_scale.requires_grad or w2_scale.requires_grad) and torch.is_grad_enabled():
         return _without_gradient("experts_w4", out, lambda: experts_w4(

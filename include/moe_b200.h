@@ -228,7 +228,7 @@ typedef struct {
 int moe_route_experts(const moe_route_experts_args* args);
 
 /* Gradient of moe_route_experts' weights: grad_w fp32 [T, top_k], the forward call's logits and idx (distinct
- * per row; values outside [0, E) take no part) -> grad_logits [T, E] contiguous, of the logits' type. */
+ * per row; values outside [0, E) take no part, and a row without a pick has a zero gradient) -> grad_logits [T, E] contiguous, of the logits' type. */
 typedef struct {
   const float* grad_w;
   const void* logits;
@@ -262,7 +262,8 @@ int moe_linear_w4(const moe_linear_w4_args* args);
  * [0, E): out[t] += w[t, j] * W2[e] (X1 * silu(X2)), [X1 | X2] = W13[e] x[t]. x [T, H] with rows x_stride
  * elements apart; idx int32 and w fp32 [T, top_k]; w13 stacked [E, 2 I, H], w2 stacked [E, H, I]; out [T, H]
  * contiguous, of x's type (zeros for a token without a pick here). w13 and w2 16-byte, the workspace 256-byte aligned; neither
- * out nor the workspace may overlap an input, nor each other; local_offset >= 0. 0 <= T <= 65535, top_k <= 32, E <= 1024, H and I up
+ * out nor the workspace may overlap an input, nor each other; local_offset >= 0. Sums in fp32, rounded once; between the products
+ * X1 * silu(X2) carries 16 bits (two bf16 terms, an error of at most 2^-17 of each value). 0 <= T <= 65535, top_k <= 32, E <= 1024, H and I up
  * to 2^30, E * H and E * 2 I below 2^31. */
 size_t moe_experts_w4_workspace_bytes(int T, int top_k, int E, int H, int I);
 typedef struct {
